@@ -61,7 +61,8 @@ EXPORTS = ["ckr_last_error", "ckr_version", "ckr_device_count", "ckr_stream_crea
            "ckr_probe_dirichlet", "ckr_probe_temperature", "ckr_probe_tau_schedule", "ckr_probe_noise_dirichlet", "ckr_probe_noise_pick",
            "ckr_gemm_nt", "ckr_conv_gemm", "ckr_conv_gemm_pieces", "ckr_split_pieces", "ckr_conv_wsplit", "ckr_conv_wgrad", "ckr_conv_wflip", "ckr_conv_bias_relu_bn", "ckr_conv_bn_relu_backward", "ckr_conv_bias_grad",
            "ckr_gemm_small", "ckr_gemm_tall", "ckr_im2col", "ckr_bn_forward", "ckr_bn_backward",
-           "ckr_policy_loss", "ckr_value_loss", "ckr_loss_sums", "ckr_adam_step", "ckr_sum_rows", "ckr_value_head_step", "ckr_policy_head_step"]
+           "ckr_policy_loss", "ckr_value_loss", "ckr_loss_sums", "ckr_adam_step", "ckr_sum_rows", "ckr_value_head_step", "ckr_policy_head_step",
+           "ckr_logprobs_scratch", "ckr_logprobs_forward", "ckr_logprobs_backward", "ckr_adamw_step", "ckr_grad_norm", "ckr_adamw_read_moments", "ckr_adamw_write_moments"]
 
 _lib = None
 
@@ -128,6 +129,14 @@ def load():
         L.ckr_engine_set_ln_table.argtypes = [vp, vp, C.c_int32]
         L.ckr_engine_game.argtypes = [vp, C.c_int32, vp, vp, vp, vp]
         L.ckr_engine_root.argtypes = [vp, C.c_int32, C.c_int32, C.POINTER(NodeInfo), C.POINTER(NodeInfo), C.POINTER(C.c_int32)]
+    L.ckr_logprobs_scratch.argtypes = [vp]
+    L.ckr_logprobs_scratch.restype = i64
+    L.ckr_logprobs_forward.argtypes = [vp, vp]
+    L.ckr_logprobs_backward.argtypes = [vp, vp]
+    L.ckr_adamw_step.argtypes = [vp, vp]
+    L.ckr_grad_norm.argtypes = [C.c_int32, vp, vp, vp, C.c_double, vp, i64, vp, vp, vp]
+    L.ckr_adamw_read_moments.argtypes = [vp, vp, vp, vp, i64, vp, vp, vp]
+    L.ckr_adamw_write_moments.argtypes = [vp, vp, i64, vp, vp, vp, vp, vp]
     L.ckr_probe_dirichlet.argtypes = [C.c_double, C.c_int32, C.c_int32, C.c_uint64, vp]
     L.ckr_probe_temperature.argtypes = [vp, C.c_int32, C.c_double, C.c_int32, C.c_uint64, vp]
     L.ckr_probe_tau_schedule.argtypes = [C.c_double, C.c_double, C.c_int32, C.c_int32, vp]

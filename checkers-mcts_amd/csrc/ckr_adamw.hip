@@ -1,0 +1,363 @@
+// ckr_adamw.hip -- one AdamW update of many tensors, with the moments in 32 or in 8 bits.
+//
+//     norm = sqrt(sum g^2) over all tensors (float64),  c = min(1, max_norm / (norm + 1e-6)),  g := c g        (where clipping is on)
+//     m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2,   t = t + 1
+//     w = w (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+// Parameters of 16 bits have a float32 master copy w; the parameter is its rounding.
+//
+// 8-bit moments: blocks of 128 elements, each with a scale byte b (the power of two 2^(b - 127), one above the block's largest value;
+// 255: the block holds a value that is not finite and reads back as NaN).  A code is a small float below that scale,
+//     m: sign, 4 exponent bits, 3 mantissa bits   value (1 + M / 8) 2^(E - 15) 2^(b - 127)
+//     v: 5 exponent bits, 3 mantissa bits         value (1 + M / 8) 2^(E - 31) 2^(b - 127)
+// code 0 is 0.  A value of v below the smallest code is raised to it: as 0 it would divide by eps alone.
+// The rounding to 3 mantissa bits is stochastic.  With 1 - b2 = 0.001, v moves by a thousandth of itself a step and a code is 1/8 to
+// 1/16 wide: to the nearest code it would not move at all, whatever the gradients.  16 dither bits per value, from Philox4x32-10 with
+// key = seed and counter = (group of 8 elements, step): whoever knows the seed can repeat a run, and graphs replay with fresh bits.
+// The moments themselves are computed in float64 on this path, so that which code a value falls to is decided by the formula and not
+// by the order of float32 operations (a v_fma_f64 issues at the rate of a v_fma_f32 here).
+#include "ckr_host.h"
+#include "ckr_device.hip.h"
+#include <cmath>
+#include <cstring>
+
+namespace ckr {
+
+constexpr int TENSORS = 96;                   // of one launch: their pointers and sizes travel in the kernel's arguments (< 4 KB)
+constexpr int CHUNK = 2048;                   // elements of one tensor that a workgroup takes at a time: 256 threads x 8
+constexpr int BLOCKS = 2048;                  // at most (8 workgroups of 256 threads on each of 256 CUs)
+constexpr int M_TOP = 15, V_TOP = 31;
+
+struct TensorTable {
+    void* p[TENSORS];
+    const void* g[TENSORS];
+    long long n[TENSORS], off[TENSORS];
+    unsigned first[TENSORS + 1];              // chunks before tensor i
+    int tensors;
+};
+static_assert(sizeof(TensorTable) <= 3600, "the table has to fit the kernel arguments beside the hyperparameters");
+
+struct Hyper {
+    float* master; void* m; void* v; uint8_t* m_scale; uint8_t* v_scale;
+    int* step; unsigned* ticket;
+    const float* d_lr; const double* norm;    // norm[0], the factor c norm[1]
+    double lr, beta1, beta2, ln_beta1, ln_beta2, weight_decay;
+    unsigned long long seed;
+    float eps;
+};
+
+// the tensor that chunk c belongs to
+__device__ __forceinline__ int tensor_of(const TensorTable& T, unsigned c) {
+    int lo = 0, hi = T.tensors;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (T.first[mid] <= c) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// ---- the 8-bit formats, on the high word of a double: 11 exponent bits, the first 20 bits of the mantissa ---------------------------
+__device__ __forceinline__ unsigned high_word(double x) { return (unsigned)__double2hiint(x) & 0x7FFFFFFFu; }
+
+// the scale byte of a block whose largest high word is h
+__device__ __forceinline__ int scale_byte(unsigned h) {
+    const int b = (int)(h >> 20) - 1023 + 1 + 127;
+    return b > 254 ? 255 : b < 1 ? 1 : b;
+}
+template <int TOP> __device__ __forceinline__ int encode(unsigned h, int scale, unsigned dither17) {      // magnitude only, <= 0: below the smallest code
+    return (int)((h + dither17) >> 17) - ((scale - 127 + 1023 - TOP) << 3);
+}
+__device__ __forceinline__ unsigned encode_m(double x, int scale, unsigned dither17) {
+    const int c = encode<M_TOP>(high_word(x), scale, dither17);
+    return c <= 0 ? 0u : (unsigned)c | (__double2hiint(x) < 0 ? 128u : 0u);
+}
+__device__ __forceinline__ unsigned encode_v(double x, int scale, unsigned dither17) {
+    const unsigned h = high_word(x);
+    const int c = encode<V_TOP>(h, scale, dither17);
+    return h == 0u ? 0u : c < 1 ? 1u : (unsigned)c;
+}
+template <int TOP> __device__ __forceinline__ double decode(unsigned c, int scale) {
+    const int h = ((int)c + ((scale - 127 + 1023 - TOP) << 3)) << 17;
+    const double x = __hiloint2double(c ? h : 0, 0);
+    return scale == 255 ? (double)__builtin_nanf("") : x;
+}
+__device__ __forceinline__ double decode_m(unsigned c, int scale) {
+    const double x = decode<M_TOP>(c & 127u, scale);
+    return c & 128u ? -x : x;
+}
+__device__ __forceinline__ double decode_v(unsigned c, int scale) { return decode<V_TOP>(c, scale); }
+
+__device__ __forceinline__ unsigned row16_max(unsigned v) {                       // over the 16 lanes (of 8 elements) of a block of 128
+    v = max(v, (unsigned)bfly_i32<1>((int)v)); v = max(v, (unsigned)bfly_i32<2>((int)v));
+    v = max(v, (unsigned)bfly_i32<4>((int)v)); v = max(v, (unsigned)bfly_i32<8>((int)v));
+    return v;
+}
+
+// ---- the update: a thread has 8 consecutive elements, 16 lanes a block of 128 --------------------------------------------------------
+template <typename T, int BITS>
+__global__ __launch_bounds__(256) void k_adamw(const TensorTable tab, const Hyper H) {
+    __shared__ unsigned last;
+    const double lr = H.d_lr ? (double)*H.d_lr : H.lr;
+    const double c = H.norm ? H.norm[1] : 1.0;
+    const float decay = (float)(1.0 - lr * H.weight_decay);
+    for (unsigned ch = blockIdx.x; ch < tab.first[tab.tensors]; ch += gridDim.x) {
+        const int i = tensor_of(tab, ch);
+        if (!tab.g[i]) continue;
+        const int t = H.step[i] + 1;
+        const double bc1 = -expm1(t * H.ln_beta1), bc2 = -expm1(t * H.ln_beta2);
+        const float rate = (float)(lr / bc1), rs = (float)(1.0 / sqrt(bc2));
+        const long long e0 = (long long)(ch - tab.first[i]) * CHUNK + threadIdx.x * 8, left = tab.n[i] - e0;
+        const long long s0 = tab.off[i] + e0;                                     // of the states: whole blocks, so never past the end
+        T* p = static_cast<T*>(tab.p[i]) + e0;
+        const T* g = static_cast<const T*>(tab.g[i]) + e0;
+        const long long blocks_end = (tab.n[i] + 127) / 128 * 128;
+        const bool in = e0 < blocks_end;
+        float w[8], gr[8], mf[8], vf[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const bool have = j < left;
+            gr[j] = have ? (float)g[j] : 0.0f;
+            w[j] = !have ? 0.0f : sizeof(T) == 4 ? (float)p[j] : H.master[s0 + j];
+        }
+        if constexpr (BITS == 32) {
+            float* m = static_cast<float*>(H.m) + s0;
+            float* v = static_cast<float*>(H.v) + s0;
+            const float b1 = (float)H.beta1, b2 = (float)H.beta2, a1 = (float)(1.0 - H.beta1), a2 = (float)(1.0 - H.beta2), cf = (float)c;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (in) {
+                    const float x = gr[j] * cf;
+                    m[j] = mf[j] = b1 * m[j] + a1 * x;
+                    v[j] = vf[j] = b2 * v[j] + a2 * x * x;
+                }
+        } else {
+            uint8_t* m = static_cast<uint8_t*>(H.m) + s0;
+            uint8_t* v = static_cast<uint8_t*>(H.v) + s0;
+            const int ms = in ? H.m_scale[s0 / 128] : 1, vs = in ? H.v_scale[s0 / 128] : 1;
+            double md[8], vd[8];
+            unsigned hm = 0, hv = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const double x = (double)gr[j] * c;
+                md[j] = H.beta1 * decode_m(in ? m[j] : 0u, ms) + (1.0 - H.beta1) * x;
+                vd[j] = H.beta2 * decode_v(in ? v[j] : 0u, vs) + (1.0 - H.beta2) * x * x;
+                hm = max(hm, high_word(md[j])); hv = max(hv, high_word(vd[j]));
+                mf[j] = (float)md[j]; vf[j] = (float)vd[j];
+            }
+            const int ms1 = scale_byte(row16_max(hm)), vs1 = scale_byte(row16_max(hv));
+            const unsigned long long grp = (unsigned long long)s0 / 8;
+            const u32x4 r = philox((unsigned)H.seed, (unsigned)(H.seed >> 32), (unsigned)grp, (unsigned)(grp >> 32), (unsigned)t, 0u);
+            const unsigned rw[4] = {r.x, r.y, r.z, r.w};
+            if (in) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {                                     // 16 of 32 random bits for v, the others for m: 2 r + 1 of 2^17
+                    const unsigned lo = rw[j >> 1] & 0xFFFFu, hi = rw[j >> 1] >> 16;
+                    m[j] = (uint8_t)encode_m(md[j], ms1, 2u * (j & 1 ? lo : hi) + 1u);
+                    v[j] = (uint8_t)encode_v(vd[j], vs1, 2u * (j & 1 ? hi : lo) + 1u);
+                }
+                if ((threadIdx.x & 15) == 0) { H.m_scale[s0 / 128] = (uint8_t)ms1; H.v_scale[s0 / 128] = (uint8_t)vs1; }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < left) {
+                const float x = w[j] * decay - rate * (mf[j] / (sqrtf(vf[j]) * rs + H.eps));
+                if constexpr (sizeof(T) == 4) p[j] = x;
+                else { H.master[s0 + j] = x; p[j] = (T)x; }
+            }
+    }
+    // The workgroup that ends last advances the step counters: by then every other one has read them.
+    __syncthreads();
+    if (!threadIdx.x) last = __hip_atomic_fetch_add(H.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    for (int i = threadIdx.x; i < tab.tensors; i += 256)
+        if (tab.g[i]) H.step[i] += 1;
+    if (!threadIdx.x) __hip_atomic_store(H.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// ---- the global norm: every workgroup's sum of squares in parts[base + blockIdx], the last of all `total` workgroups adds them in order --
+template <typename T>
+__global__ __launch_bounds__(256) void k_grad_norm(const TensorTable tab, double max_norm, double* __restrict__ parts, int base, int total,
+                                                   unsigned* __restrict__ ticket, double* __restrict__ out) {
+    __shared__ double red[256];
+    __shared__ unsigned last;
+    double s = 0.0;
+    for (unsigned ch = blockIdx.x; ch < tab.first[tab.tensors]; ch += gridDim.x) {
+        const int i = tensor_of(tab, ch);
+        if (!tab.g[i]) continue;
+        const long long e0 = (long long)(ch - tab.first[i]) * CHUNK + threadIdx.x * 8, left = tab.n[i] - e0;
+        const T* g = static_cast<const T*>(tab.g[i]) + e0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < left) { const double x = (double)(float)g[j]; s += x * x; }
+    }
+    red[threadIdx.x] = s;
+    __syncthreads();
+    for (int d = 128; d >= 1; d >>= 1) { if ((int)threadIdx.x < d) red[threadIdx.x] += red[threadIdx.x + d]; __syncthreads(); }
+    // the part travels as a device-scope atomic and has been acknowledged before the ticket is taken: no cache is written back for it
+    if (!threadIdx.x) {
+        __hip_atomic_store(parts + base + blockIdx.x, red[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __builtin_amdgcn_s_waitcnt(0);
+        last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)total - 1u;
+    }
+    __syncthreads();
+    if (!last) return;
+    s = 0.0;
+    for (int b = threadIdx.x; b < total; b += 256) s += __hip_atomic_load(parts + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    red[threadIdx.x] = s;
+    __syncthreads();
+    for (int d = 128; d >= 1; d >>= 1) { if ((int)threadIdx.x < d) red[threadIdx.x] += red[threadIdx.x + d]; __syncthreads(); }
+    if (threadIdx.x) return;
+    const double norm = sqrt(red[0]), c = max_norm / (norm + 1e-6);
+    out[0] = norm;
+    out[1] = c >= 1.0 ? 1.0 : c;                                                  // NaN stays NaN
+    __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// ---- reading and writing 8-bit moments (n a multiple of 128) -------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void k_moments_read(const uint8_t* __restrict__ m, const uint8_t* __restrict__ v, const uint8_t* __restrict__ m_scale,
+                                                      const uint8_t* __restrict__ v_scale, long long n, float* __restrict__ m_out, float* __restrict__ v_out) {
+    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (long long)gridDim.x * 2048)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            m_out[i + j] = (float)decode_m(m[i + j], m_scale[i / 128]);
+            v_out[i + j] = (float)decode_v(v[i + j], v_scale[i / 128]);
+        }
+}
+__global__ __launch_bounds__(256) void k_moments_write(const float* __restrict__ m_in, const float* __restrict__ v_in, long long n, uint8_t* __restrict__ m,
+                                                       uint8_t* __restrict__ v, uint8_t* __restrict__ m_scale, uint8_t* __restrict__ v_scale) {
+    // whole blocks of 128 are whole rows of 16 lanes: the lanes of a row take part in its maximum together
+    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (long long)gridDim.x * 2048) {
+        unsigned hm = 0, hv = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { hm = max(hm, high_word((double)m_in[i + j])); hv = max(hv, high_word((double)v_in[i + j])); }
+        const int ms = scale_byte(row16_max(hm)), vs = scale_byte(row16_max(hv));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {                                             // to nearest: half a step is 2^16 of 2^17
+            m[i + j] = (uint8_t)encode_m((double)m_in[i + j], ms, 0x10000u);
+            v[i + j] = (uint8_t)encode_v((double)v_in[i + j], vs, 0x10000u);
+        }
+        if ((threadIdx.x & 15) == 0) { m_scale[i / 128] = (uint8_t)ms; v_scale[i / 128] = (uint8_t)vs; }
+    }
+}
+
+// tensors [k, k + TENSORS) of the call
+static void fill_table(TensorTable& T, int count, int k, const int64_t* sizes, const int64_t* offsets, void* const* params, const void* const* grads) {
+    T.tensors = count - k < TENSORS ? count - k : TENSORS;
+    unsigned chunks = 0;
+    for (int i = 0; i < T.tensors; ++i) {
+        T.p[i] = params ? params[k + i] : nullptr;
+        T.g[i] = grads[k + i];
+        T.n[i] = sizes[k + i];
+        T.off[i] = offsets ? offsets[k + i] : 0;
+        T.first[i] = chunks;
+        chunks += T.g[i] ? (unsigned)((sizes[k + i] + CHUNK - 1) / CHUNK) : 0u;
+    }
+    T.first[T.tensors] = chunks;
+}
+static unsigned grid_of(const TensorTable& T) { const unsigned c = T.first[T.tensors]; return c < 1u ? 1u : c < (unsigned)BLOCKS ? c : (unsigned)BLOCKS; }
+
+static int check_tensors(const char* who, int count, const int64_t* sizes, const void* const* grads, int dtype) {
+    if (count <= 0 || !sizes || !grads) return fail(CKR_ERR_INVALID, "%s: no tensors", who);
+    if (dtype < CKR_F32 || dtype > CKR_F16) return fail(CKR_ERR_INVALID, "%s: unknown type %d", who, dtype);
+    for (int i = 0; i < count; ++i)
+        if (sizes[i] < 1 || sizes[i] > (1ll << 36)) return fail(CKR_ERR_INVALID, "%s: tensor %d has %lld elements: 1 .. 2^36", who, i, (long long)sizes[i]);
+    return CKR_OK;
+}
+
+}  // namespace ckr
+
+extern "C" {
+
+int ckr_adamw_step(const ckr_adamw_args* a, void* stream) {
+    using namespace ckr;
+    if (!a) return fail(CKR_ERR_INVALID, "ckr_adamw_step: null argument");
+    if (int rc = check_tensors("ckr_adamw_step", a->count, a->sizes, a->grads, a->dtype)) return rc;
+    if (!a->offsets || !a->params || !a->m || !a->v || !a->d_step || !a->d_ticket) return fail(CKR_ERR_INVALID, "ckr_adamw_step: null pointer");
+    if (a->state_bits != 32 && a->state_bits != 8) return fail(CKR_ERR_INVALID, "ckr_adamw_step: states have 32 or 8 bits");
+    if (a->state_bits == 8 && (!a->m_scale || !a->v_scale)) return fail(CKR_ERR_INVALID, "ckr_adamw_step: 8-bit states need their scales");
+    if (a->dtype != CKR_F32 && !a->master) return fail(CKR_ERR_INVALID, "ckr_adamw_step: parameters of 16 bits need a master copy");
+    if (!(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0) || !(a->eps > 0.0f)) return fail(CKR_ERR_INVALID, "ckr_adamw_step: betas in [0, 1), eps > 0");
+    for (int i = 0; i < a->count; ++i) {
+        if (a->grads[i] && !a->params[i]) return fail(CKR_ERR_INVALID, "ckr_adamw_step: tensor %d has a gradient and no parameter", i);
+        if (a->offsets[i] < 0 || a->offsets[i] % 128) return fail(CKR_ERR_INVALID, "ckr_adamw_step: offsets are multiples of 128");
+    }
+    if (int rc = require_device()) return rc;
+    hipStream_t s = (hipStream_t)stream;
+    for (int k = 0; k < a->count; k += TENSORS) {
+        TensorTable T;
+        fill_table(T, a->count, k, a->sizes, a->offsets, a->params, a->grads);
+        if (!T.first[T.tensors]) continue;
+        const Hyper H = {a->master, a->m, a->v, a->m_scale, a->v_scale, a->d_step + k, a->d_ticket, a->d_lr, a->d_norm, a->lr, a->beta1, a->beta2,
+                         std::log(a->beta1), std::log(a->beta2), a->weight_decay, (unsigned long long)a->seed, a->eps};
+        const dim3 grid(grid_of(T)), block(256);
+#define CKR_ADAMW(TYPE)                                                                                       \
+        do {                                                                                                  \
+            if (a->state_bits == 32) hipLaunchKernelGGL((k_adamw<TYPE, 32>), grid, block, 0, s, T, H);         \
+            else hipLaunchKernelGGL((k_adamw<TYPE, 8>), grid, block, 0, s, T, H);                              \
+        } while (0)
+        if (a->dtype == CKR_F32) CKR_ADAMW(float);
+        else if (a->dtype == CKR_BF16) CKR_ADAMW(__bf16);
+        else CKR_ADAMW(_Float16);
+#undef CKR_ADAMW
+        CKR_HIP(hipGetLastError());
+    }
+    return CKR_OK;
+}
+
+int ckr_grad_norm(int32_t count, const int64_t* sizes, const void* const* grads, const int32_t* dtypes, double max_norm, double* d_parts, int64_t parts,
+                  uint32_t* d_ticket, double* d_out, void* stream) {
+    using namespace ckr;
+    if (int rc = check_tensors("ckr_grad_norm", count, sizes, grads, CKR_F32)) return rc;
+    if (!dtypes || !d_parts || !d_ticket || !d_out || !(max_norm > 0.0)) return fail(CKR_ERR_INVALID, "ckr_grad_norm: bad argument");
+    // launches: runs of tensors of one type, at most TENSORS each
+    int64_t total = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        int64_t base = 0;
+        for (int k = 0; k < count;) {
+            int end = k;
+            while (end < count && end - k < TENSORS && dtypes[end] == dtypes[k]) ++end;
+            if (dtypes[k] < CKR_F32 || dtypes[k] > CKR_F16) return fail(CKR_ERR_INVALID, "ckr_grad_norm: unknown type %d", (int)dtypes[k]);
+            TensorTable T;
+            fill_table(T, end, k, sizes, nullptr, nullptr, grads);
+            const unsigned grid = grid_of(T);
+            if (pass) {
+                hipStream_t s = (hipStream_t)stream;
+                if (dtypes[k] == CKR_F32) hipLaunchKernelGGL((k_grad_norm<float>), dim3(grid), dim3(256), 0, s, T, max_norm, d_parts, (int)base, (int)total, d_ticket, d_out);
+                else if (dtypes[k] == CKR_BF16) hipLaunchKernelGGL((k_grad_norm<__bf16>), dim3(grid), dim3(256), 0, s, T, max_norm, d_parts, (int)base, (int)total, d_ticket, d_out);
+                else hipLaunchKernelGGL((k_grad_norm<_Float16>), dim3(grid), dim3(256), 0, s, T, max_norm, d_parts, (int)base, (int)total, d_ticket, d_out);
+                CKR_HIP(hipGetLastError());
+            }
+            base += grid;
+            k = end;
+        }
+        if (!pass) {
+            total = base;
+            if (total > parts) return fail(CKR_ERR_INVALID, "ckr_grad_norm: %lld partial sums, room for %lld", (long long)total, (long long)parts);
+            if (int rc = require_device()) return rc;
+        }
+    }
+    return CKR_OK;
+}
+
+int ckr_adamw_read_moments(const uint8_t* m, const uint8_t* v, const uint8_t* m_scale, const uint8_t* v_scale, int64_t n, float* m_out, float* v_out, void* stream) {
+    using namespace ckr;
+    if (!m || !v || !m_scale || !v_scale || !m_out || !v_out || n <= 0 || n % 128) return fail(CKR_ERR_INVALID, "ckr_adamw_read_moments: bad argument");
+    if (int rc = require_device()) return rc;
+    const long long blocks = (n + 2047) / 2048;
+    hipLaunchKernelGGL(k_moments_read, dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, (hipStream_t)stream, m, v, m_scale, v_scale, (long long)n, m_out, v_out);
+    CKR_HIP(hipGetLastError());
+    return CKR_OK;
+}
+
+int ckr_adamw_write_moments(const float* m_in, const float* v_in, int64_t n, uint8_t* m, uint8_t* v, uint8_t* m_scale, uint8_t* v_scale, void* stream) {
+    using namespace ckr;
+    if (!m || !v || !m_scale || !v_scale || !m_in || !v_in || n <= 0 || n % 128) return fail(CKR_ERR_INVALID, "ckr_adamw_write_moments: bad argument");
+    if (int rc = require_device()) return rc;
+    const long long blocks = (n + 2047) / 2048;
+    hipLaunchKernelGGL(k_moments_write, dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, (hipStream_t)stream, m_in, v_in, (long long)n, m, v, m_scale, v_scale);
+    CKR_HIP(hipGetLastError());
+    return CKR_OK;
+}
+
+}  // extern "C"

@@ -43,19 +43,24 @@ class PolicyValueNet(nn.Module):
     def _block(blk, x):
         return blk["bn"](F.relu(blk["conv"](x)))
 
-    def forward(self, x):
+    def logits(self, x):
         """x: [B,14,8,8] (any memory format; channels-last is free for the
-        engine's NHWC buffer).  Returns (p [B,512] float32 softmax, v [B] float32)."""
+        engine's NHWC buffer).  Returns (policy logits [B,512], v [B] float32)."""
         for blk in self.body:
             x = self._block(blk, x)
         p = self._block(self.pol2, self._block(self.pol1, x))
         p = p.permute(0, 2, 3, 1).reshape(p.shape[0], 512)          # Keras Flatten: (H, W, C)
-        p = F.softmax(self.pol_fc(p).float(), dim=1)
+        p = self.pol_fc(p)
         v = self._block(self.val1, x)
         v = v.permute(0, 2, 3, 1).reshape(v.shape[0], 64)
         v = self.val_bn(F.relu(self.val_fc1(v)))
         v = torch.tanh(self.val_fc2(v).float()).reshape(-1)
         return p, v
+
+    def forward(self, x):
+        """x as for `logits`.  Returns (p [B,512] float32 softmax, v [B] float32)."""
+        z, v = self.logits(x)
+        return F.softmax(z.float(), dim=1), v
 
     def keras_init(self, seed=0):
         g = torch.Generator().manual_seed(seed)

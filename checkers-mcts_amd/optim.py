@@ -1,0 +1,296 @@
+"""AdamW over many tensors in one launch, with moments in 32 or in 8 bits (csrc/ckr_adamw.hip).
+
+The reference trains with Keras' Adam (training_pipeline.py:113), which `train_hip.HipTrainStep` has for the 128-kernel network in
+float32.  This optimiser takes any module's parameters, in float32, bfloat16 or float16; `train.train_nn` uses it under OPTIMIZER.
+"""
+import ctypes as C
+import math
+
+import torch
+
+from . import _lib
+
+BLOCK = 128                         # elements that share a scale in 8-bit moments; every tensor's part of the states is padded to it
+TENSORS, BLOCKS = 96, 2048          # of one launch (ckr_adamw.hip)
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class AdamWArgs(C.Structure):
+    """ckr_adamw_args (include/ckr.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("sizes", "offsets", "params", "grads", "master", "m", "v", "m_scale", "v_scale",
+                                          "d_step", "d_ticket", "d_lr", "d_norm")] + \
+        [(n, C.c_double) for n in ("lr", "beta1", "beta2", "weight_decay")] + [("seed", C.c_uint64), ("eps", C.c_float)] + \
+        [(n, C.c_int32) for n in ("count", "dtype", "state_bits")]
+
+
+def _layout(t):
+    """Strides of the dimensions that have more than one element; None unless the tensor fills its memory without gaps or overlaps."""
+    dims = [(st, n) for n, st in zip(t.shape, t.stride()) if n > 1]
+    want = 1
+    for st, n in sorted(dims):
+        if st != want:
+            return None
+        want *= n
+    return dims
+
+
+class _Batch:
+    """The tensors of one group and type: what one call of ckr_adamw_step takes."""
+
+    def __init__(self, group, dtype, params, offsets, first):
+        n = len(params)
+        self.group, self.dtype, self.params, self.first, self.n = group, dtype, params, first, n
+        self.layouts = [_layout(p) for p in params]
+        self.strides = [p.stride() for p in params]
+        self.shapes = [p.shape for p in params]
+        self.sizes = (C.c_int64 * n)(*[p.numel() for p in params])
+        self.offsets = (C.c_int64 * n)(*offsets)
+
+
+class AdamW:
+    """AdamW with decoupled weight decay:
+
+        m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  w = w (1 - lr weight_decay) - lr m^ / (sqrt(v^) + eps)
+
+    with m^, v^ the bias-corrected moments and every tensor's own step count (a tensor without a gradient is left alone).
+
+    params        tensors, or groups {"params": [...], "lr": ..., "betas": ..., "eps": ..., "weight_decay": ...}, of float32, bfloat16
+                  or float16 on one GPU, dense in memory (any order of dimensions).  16-bit parameters get a float32 master copy, which is
+                  what the optimiser updates; the parameter is its rounding.
+    lr            a number, or a float32 device scalar (read by the kernel: a captured step follows its changes).
+    state_bits    32, or 8: a byte for each moment and a scale byte for each 128 elements, rounded stochastically (seed).
+    max_norm      clip the gradients by their global norm (over all groups): g * min(1, max_norm / (norm + 1e-6)); the norm of the last
+                  step is `grad_norm`, a float64 device scalar.
+
+    step() runs on the current stream and does not synchronise; it can be captured into a HIP graph (gradients then have to stay where
+    they are: zero_grad(set_to_none=False)).  Steps of one optimiser must not run at the same time."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_norm=None, seed=0):
+        if state_bits not in (32, 8):
+            raise ValueError("state_bits must be 32 or 8, got %r" % (state_bits,))
+        if max_norm is not None and not (0 < float(max_norm) < math.inf):
+            raise ValueError("max_norm must be positive and finite, got %r" % (max_norm,))
+        if isinstance(params, torch.Tensor):
+            raise ValueError("params must be a list of tensors or of groups, got a tensor")
+        params = list(params)
+        groups = [dict(g) for g in params] if params and isinstance(params[0], dict) else [{"params": params}]
+        for g in groups:
+            g["params"] = [g["params"]] if isinstance(g["params"], torch.Tensor) else list(g["params"])
+            for k, dflt in (("lr", lr), ("betas", betas), ("eps", eps), ("weight_decay", weight_decay)):
+                g.setdefault(k, dflt)
+        self.param_groups, self.state_bits, self.max_norm, self.seed = groups, int(state_bits), None if max_norm is None else float(max_norm), int(seed) & (2 ** 64 - 1)
+        every = [p for g in groups for p in g["params"]]
+        if not every:
+            raise ValueError("AdamW: no parameters")
+        for p in every:
+            if not isinstance(p, torch.Tensor) or not p.is_cuda or p.dtype not in DTYPES or p.device != every[0].device:
+                raise ValueError("parameters must be float32, bfloat16 or float16 tensors on one GPU")
+            if not p.is_leaf:
+                raise ValueError("AdamW steps leaf tensors only")
+            if _layout(p) is None:
+                raise ValueError("a parameter of shape %s and strides %s does not fill its memory" % (list(p.shape), list(p.stride())))
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in every if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("parameters share memory (or one is listed twice)")
+        for g in groups:
+            self._check_group(g)
+        self.device = dev = every[0].device
+        # the states: one flat buffer a moment, tensor i at offsets[i]
+        self.params, self.offsets, total = every, [], 0
+        for p in every:
+            self.offsets.append(total)
+            total += (p.numel() + BLOCK - 1) // BLOCK * BLOCK
+        self.total = total
+        where = {id(p): o for p, o in zip(every, self.offsets)}
+        self._batches, first = [], 0
+        for g in groups:
+            for dtype in DTYPES:
+                mine = [p for p in g["params"] if p.dtype == dtype and p.numel()]
+                if mine:
+                    self._batches.append(_Batch(g, dtype, mine, [where[id(p)] for p in mine], first))
+                    first += len(mine)
+        state = torch.uint8 if self.state_bits == 8 else torch.float32
+        z = lambda n, dtype: torch.zeros((n,), dtype=dtype, device=dev)
+        self.exp_avg, self.exp_avg_sq = z(total, state), z(total, state)
+        self.scales = (torch.ones((2, max(1, total // BLOCK)), dtype=torch.uint8, device=dev)) if self.state_bits == 8 else None
+        self.master = None
+        if any(p.dtype != torch.float32 for p in every):
+            self.master = z(total, torch.float32)
+            for p, o in zip(every, self.offsets):
+                if p.dtype != torch.float32:
+                    self._flat_view(self.master, p, o).copy_(p.detach())
+        self.steps = z(max(1, first), torch.int32)                     # in the order of the batches
+        self._ticket = z(2, torch.int32)
+        # partial sums of the norm: one launch for each run of up to TENSORS tensors of one type
+        launches = sum((b.n + TENSORS - 1) // TENSORS for b in self._batches)
+        self._parts, self._norm = (z(max(1, launches) * BLOCKS, torch.float64), z(2, torch.float64)) if self.max_norm is not None else (None, None)
+        self._sizes_all = (C.c_int64 * first)(*[n for b in self._batches for n in b.sizes])
+        self._dtypes_all = (C.c_int32 * first)(*[DTYPES[b.dtype] for b in self._batches for _ in range(b.n)])
+        self._streams = {torch.cuda.current_stream(dev).cuda_stream}
+        torch.cuda.current_stream(dev).synchronize()                   # a step on any stream finds the states in place
+        self._L = _lib.load()
+
+    def _check_group(self, g):
+        lr = g["lr"]
+        if isinstance(lr, torch.Tensor):
+            if not lr.is_cuda or lr.dtype != torch.float32 or lr.numel() != 1:
+                raise ValueError("lr must be a number or a float32 device scalar")
+        elif not 0 <= float(lr) < math.inf:
+            raise ValueError("lr must be finite and not negative, got %r" % (lr,))
+        b1, b2 = g["betas"]
+        if not (0 <= b1 < 1 and 0 <= b2 < 1):
+            raise ValueError("betas must be in [0, 1), got %r" % (g["betas"],))
+        if not 1e-37 <= float(g["eps"]) <= 1e30:
+            raise ValueError("eps must be positive (1e-37 to 1e30), got %r" % (g["eps"],))
+        if not 0 <= float(g["weight_decay"]) < math.inf:
+            raise ValueError("weight_decay must be finite and not negative, got %r" % (g["weight_decay"],))
+
+    @staticmethod
+    def _flat_view(flat, p, offset):
+        """p's part of a flat buffer, in p's own shape and order of dimensions."""
+        return flat.as_strided(p.shape, p.stride(), flat.storage_offset() + offset) if p.numel() else flat.new_empty(p.shape)
+
+    def _gradients(self, b, keep):
+        """Device pointers of a batch's parameters and gradients (0: none); a gradient that lies otherwise than its parameter is copied."""
+        ps, gs = [], []
+        for p, strides, shape, layout in zip(b.params, b.strides, b.shapes, b.layouts):
+            g = p.grad
+            if g is None:
+                ps.append(0)
+                gs.append(0)
+                continue
+            if p.stride() != strides or p.shape != shape or p.dtype != b.dtype or p.device != self.device:
+                raise ValueError("a parameter's shape, strides, type or device changed after the optimiser was made")
+            if g.stride() != strides:
+                if g.layout != torch.strided:
+                    raise ValueError("sparse gradients are not supported")
+                if g.shape != shape:
+                    raise ValueError("a gradient of shape %s for a parameter of shape %s" % (list(g.shape), list(shape)))
+                if _layout(g) != layout:
+                    g = torch.empty_strided(shape, strides, dtype=b.dtype, device=self.device).copy_(g)
+                    keep.append(g)
+            if g.dtype != b.dtype or g.device != self.device:
+                raise ValueError("a gradient must have its parameter's type and device")
+            ps.append(p.data_ptr())
+            gs.append(g.data_ptr())
+        return (C.c_void_p * b.n)(*ps), (C.c_void_p * b.n)(*gs)
+
+    @torch.no_grad()
+    def step(self):
+        """One update of every parameter that has a gradient."""
+        if torch.cuda.current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self._step()
+        return self._step()
+
+    def _step(self):
+        L = self._L
+        cur = torch.cuda.current_stream(self.device)
+        s = cur.cuda_stream
+        if s not in self._streams:                                     # the allocator has to know before it hands the memory on
+            self._streams.add(s)
+            for t in (self.exp_avg, self.exp_avg_sq, self.scales, self.master, self.steps, self._ticket, self._parts, self._norm):
+                if t is not None:
+                    t.record_stream(cur)
+        keep, ptrs = [], []
+        for b in self._batches:
+            self._check_group(b.group)
+            ptrs.append(self._gradients(b, keep))
+        if self.max_norm is not None:
+            grads = (C.c_void_p * len(self._sizes_all))(*[g for _, gs in ptrs for g in gs])
+            _lib.check(L.ckr_grad_norm(len(grads), self._sizes_all, grads, self._dtypes_all, self.max_norm, self._parts.data_ptr(),
+                                       self._parts.numel(), self._ticket.data_ptr() + 4, self._norm.data_ptr(), s))
+        scales = (None, None) if self.scales is None else (self.scales[0].data_ptr(), self.scales[1].data_ptr())
+        done = []
+        for b, (ps, gs) in zip(self._batches, ptrs):
+            g = b.group
+            lr, (b1, b2) = g["lr"], g["betas"]
+            on_device = isinstance(lr, torch.Tensor)
+            a = AdamWArgs(C.addressof(b.sizes), C.addressof(b.offsets), C.addressof(ps), C.addressof(gs),
+                          None if self.master is None else self.master.data_ptr(), self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), *scales,
+                          self.steps.data_ptr() + 4 * b.first, self._ticket.data_ptr(), lr.data_ptr() if on_device else None,
+                          None if self._norm is None else self._norm.data_ptr(), 0.0 if on_device else float(lr), float(b1), float(b2),
+                          float(g["weight_decay"]), self.seed, float(g["eps"]), b.n, DTYPES[b.dtype], self.state_bits)
+            _lib.check(L.ckr_adamw_step(C.byref(a), s))
+            done += [p for p, ptr in zip(b.params, gs) if ptr]
+        if done:
+            torch.autograd.graph.increment_version(done)               # a backward pass over what it saved before the step is refused
+
+    @property
+    def grad_norm(self):
+        """The global norm of the last step's gradients before clipping (float64 device scalar; None without max_norm)."""
+        return None if self._norm is None else self._norm[0]
+
+    def zero_grad(self, set_to_none=True):
+        grads = [p.grad for p in self.params if p.grad is not None]
+        if set_to_none:
+            for p in self.params:
+                p.grad = None
+        elif grads:
+            with torch.no_grad():
+                torch._foreach_zero_(grads)
+
+    # ---- states ---------------------------------------------------------------------------------------------
+    def moments(self):
+        """(m, v) as float32 flat tensors, tensor i at offsets[i] (split() has the views); with 32-bit states the states themselves, with
+        8 bits the values that the codes stand for."""
+        if self.state_bits == 32:
+            return self.exp_avg, self.exp_avg_sq
+        m, v = (torch.empty((self.total,), dtype=torch.float32, device=self.device) for _ in range(2))
+        if self.total:
+            with torch.cuda.device(self.device):
+                _lib.check(self._L.ckr_adamw_read_moments(self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), self.scales[0].data_ptr(), self.scales[1].data_ptr(),
+                                                          self.total, m.data_ptr(), v.data_ptr(), torch.cuda.current_stream(self.device).cuda_stream))
+        return m, v
+
+    def split(self, flat):
+        """Views of a flat tensor of moments (or of `master`), one for each parameter, in its shape."""
+        return [self._flat_view(flat, p, o) for p, o in zip(self.params, self.offsets)]
+
+    @torch.no_grad()
+    def load_moments(self, exp_avg, exp_avg_sq, step):
+        """Moments from float32 values (flat, as moments() gives them, or a list of tensors like the parameters) after `step` steps; with 8-bit
+        states to the nearest codes."""
+        flat = []
+        for given in (exp_avg, exp_avg_sq):
+            if isinstance(given, torch.Tensor):
+                if given.shape != (self.total,) or given.dtype != torch.float32 or given.device != self.device:
+                    raise ValueError("moments must be float32 [%d] on %s" % (self.total, self.device))
+                flat.append(given.contiguous())
+            else:
+                given = list(given)
+                if len(given) != len(self.params) or any(t.shape != p.shape for t, p in zip(given, self.params)):
+                    raise ValueError("moments must have the parameters' shapes")
+                buf = torch.zeros((self.total,), dtype=torch.float32, device=self.device)
+                for view, t in zip(self.split(buf), given):
+                    view.copy_(t)
+                flat.append(buf)
+        if self.state_bits == 32:
+            self.exp_avg.copy_(flat[0])
+            self.exp_avg_sq.copy_(flat[1])
+        elif self.total:
+            with torch.cuda.device(self.device):
+                _lib.check(self._L.ckr_adamw_write_moments(flat[0].data_ptr(), flat[1].data_ptr(), self.total, self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(),
+                                                           self.scales[0].data_ptr(), self.scales[1].data_ptr(), torch.cuda.current_stream(self.device).cuda_stream))
+        self.steps.fill_(int(step))
+
+    def state_dict(self):
+        """States (the buffers themselves) and hyperparameters; load_state_dict() of an optimiser over the same parameters takes it."""
+        return {"state_bits": self.state_bits, "seed": self.seed, "exp_avg": self.exp_avg, "exp_avg_sq": self.exp_avg_sq, "scales": self.scales,
+                "master": self.master, "steps": self.steps, "sizes": [p.numel() for p in self.params],
+                "param_groups": [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups]}
+
+    @torch.no_grad()
+    def load_state_dict(self, state):
+        if state["state_bits"] != self.state_bits or state["sizes"] != [p.numel() for p in self.params] or len(state["param_groups"]) != len(self.param_groups) \
+                or (state["master"] is None) != (self.master is None) or state["steps"].numel() != self.steps.numel():
+            raise ValueError("the state belongs to other parameters, groups or state_bits")
+        for g, new in zip(self.param_groups, state["param_groups"]):
+            self._check_group(dict(g, **new))
+        for mine, other in ((self.exp_avg, state["exp_avg"]), (self.exp_avg_sq, state["exp_avg_sq"]), (self.scales, state["scales"]),
+                            (self.master, state["master"]), (self.steps, state["steps"])):
+            if mine is not None:
+                mine.copy_(other)
+        self.seed = state["seed"]
+        for g, new in zip(self.param_groups, state["param_groups"]):
+            g.update(new)

@@ -1,0 +1,193 @@
+"""What a policy says about given actions: log probabilities, entropy and top alternatives of rows of logits, with their gradient
+(csrc/ckr_logprobs.hip), and the moves a network would consider in given positions.
+
+The reference reads its policy as one dense masked softmax (Checkers.predict, Checkers.py:425-438; `rules.mask_renorm`); it has no
+counterpart of these.  All tensors live on a `cuda` (HIP) device; there is no CPU fallback.
+"""
+import ctypes as C
+from collections import namedtuple
+
+import torch
+
+from . import _lib, rules
+
+ACTIONS = 512                       # of the Checkers policy: 64 layer + 8 x + y (Checkers.py:434)
+MOST = 64                           # given actions and alternatives of a row (CKR_LOGPROBS_MOST)
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MASK_NONE, MASK_BYTES, MASK_LEGAL = 0, 1, 2
+
+ActionLogprobs = namedtuple("ActionLogprobs", "logp entropy top_action top_logp")
+RankedMoves = namedtuple("RankedMoves", "action logp entropy value")
+
+
+class LogprobsArgs(C.Structure):
+    """ckr_logprobs_args (include/ckr.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("logits", "actions", "mask", "logp", "entropy", "top_action", "top_logp", "stats",
+                                          "g_logp", "g_entropy", "grad", "scratch")] + \
+        [(n, C.c_int64) for n in ("n", "v", "row_stride", "mask_stride", "grad_stride", "scratch_bytes")] + \
+        [(n, C.c_int32) for n in ("dtype", "mask_kind", "action_bytes", "n_given", "top")] + [("inv_temperature", C.c_float)]
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _args(x, actions, mask, mask_kind, top, inv_temperature):
+    n, v = x.shape
+    a = LogprobsArgs()
+    a.logits, a.n, a.v, a.row_stride, a.dtype = x.data_ptr(), n, v, x.stride(0) if n > 1 else v, DTYPES[x.dtype]
+    if actions is not None:
+        a.actions, a.action_bytes, a.n_given = actions.data_ptr(), actions.element_size(), actions.shape[1]
+    if mask is not None:
+        a.mask, a.mask_kind, a.mask_stride = mask.data_ptr(), mask_kind, mask.stride(0) if mask.shape[0] > 1 else 0
+    a.top, a.inv_temperature = top, inv_temperature
+    return a
+
+
+def _call(fn, args, device):
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        _lib.check(fn(C.byref(args), stream))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(C.byref(args), stream))
+
+
+def _forward(x, actions, mask, mask_kind, top, inv_temperature, want_stats):
+    """x [n, v] (last dimension dense), actions [n, k] or None, mask [n or 1, ...] or None."""
+    L, n, dev = _lib.load(), x.shape[0], x.device
+    logp = None if actions is None else torch.empty(actions.shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty((n,), dtype=torch.float32, device=dev)
+    top_action = torch.empty((n, top), dtype=torch.int64, device=dev) if top else None
+    top_logp = torch.empty((n, top), dtype=torch.float32, device=dev) if top else None
+    stats = torch.empty((n, 4), dtype=torch.float32, device=dev) if want_stats else None
+    a = _args(x, actions, mask, mask_kind, top, inv_temperature)
+    a.logp, a.entropy, a.top_action, a.top_logp, a.stats = _ptr(logp), entropy.data_ptr(), _ptr(top_action), _ptr(top_logp), _ptr(stats)
+    a.scratch_bytes = L.ckr_logprobs_scratch(C.byref(a))
+    if a.scratch_bytes < 0:
+        _lib.check(int(a.scratch_bytes))
+    scratch = torch.empty((a.scratch_bytes,), dtype=torch.uint8, device=dev) if a.scratch_bytes else None
+    a.scratch = _ptr(scratch)
+    _call(L.ckr_logprobs_forward, a, dev)
+    return logp, entropy, top_action, top_logp, stats
+
+
+class _Logprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, actions, mask, mask_kind, top, inv_temperature):
+        logp, entropy, top_action, top_logp, stats = _forward(x, actions, mask, mask_kind, top, inv_temperature, True)
+        ctx.save_for_backward(x, actions, mask, stats)
+        ctx.mask_kind, ctx.inv_temperature = mask_kind, inv_temperature
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*(t for t in (top_action, top_logp) if t is not None))
+        return logp, entropy, top_action, top_logp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logp, g_entropy, _action, _top):
+        if g_logp is None and g_entropy is None:
+            return (None,) * 6
+        x, actions, mask, stats = ctx.saved_tensors
+        if g_logp is None:
+            actions = None
+        grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        g_logp, g_entropy = (None if g is None else g.float().contiguous() for g in (g_logp, g_entropy))
+        a = _args(x, actions, mask, ctx.mask_kind, 0, ctx.inv_temperature)
+        a.stats, a.g_logp, a.g_entropy, a.grad, a.grad_stride = stats.data_ptr(), _ptr(g_logp), _ptr(g_entropy), grad.data_ptr(), x.shape[1]
+        _call(_lib.load().ckr_logprobs_backward, a, x.device)
+        return (grad,) + (None,) * 5
+
+
+def _check_mask(mask, lead, v, device):
+    """-> (mask with one row or a row per row of logits, kind)."""
+    if not isinstance(mask, torch.Tensor) or mask.device != device:
+        raise ValueError("mask must be a tensor on %s" % device)
+    if mask.dtype == torch.int32:
+        width, kind = 8, MASK_LEGAL
+        if v != ACTIONS:
+            raise ValueError("legal-move words (int32 [..., 8]) belong to logits of %d actions, not %d" % (ACTIONS, v))
+    elif mask.dtype in (torch.bool, torch.uint8):
+        width, kind = v, MASK_BYTES
+    else:
+        raise ValueError("mask must be a bool tensor [..., %d] (True: allowed) or the int32 [..., 8] legal-move words of rules.movegen" % v)
+    if mask.dim() < 1 or mask.shape[-1] != width:
+        raise ValueError("the mask's last dimension must be %d, got %s" % (width, list(mask.shape)))
+    if mask.shape[:-1].numel() == 1:
+        mask = mask.reshape(1, width)
+    else:
+        try:
+            mask = mask.expand(lead + (width,)).reshape(-1, width)
+        except RuntimeError:
+            raise ValueError("a mask of shape %s does not fit logits of shape %s" % (list(mask.shape), list(lead + (v,)))) from None
+    return mask if mask.stride(1) == 1 or width == 1 else mask.contiguous(), kind
+
+
+def action_logprobs(logits, actions=None, mask=None, top=0, temperature=1.0):
+    """Log probabilities of given actions, the entropy and the top alternatives of softmax(logits / temperature).
+
+    logits    [..., V] float32, bfloat16 or float16 on the GPU, V from 1 to 2^30.  Rows may lie apart (any row stride, also 0) and start
+              anywhere; a last dimension that is not dense is copied once.
+    actions   int64 or int32, [...] (one given action a row) or [..., K] with K <= 64; a negative action is none (log p 0, no
+              gradient); one >= V gives NaN, and a NaN gradient in its row.
+    mask      the actions that count: bool [..., V], [V] or broadcastable (True: allowed), or the int32 [..., 8] legal-move words of
+              `rules.movegen` (V = 512).  A logit of -inf is masked too; what is masked may hold anything, NaN included.
+    top       up to 64 alternatives: the most likely allowed actions, ties to the lower action.
+
+    Returns ActionLogprobs(logp, entropy, top_action, top_logp), float32 and int64 (None for what was not asked).  A masked action has log p
+    -inf.  A row without an allowed action: log p -inf, entropy 0, gradient 0.  Where there are fewer than `top` alternatives: action
+    -1, log p -inf.  NaN or +inf among the allowed logits make the row's numbers NaN and its alternatives -1.
+
+    Differentiable (once) in logits through logp and entropy; the alternatives are not.  A masked given action of a row with others keeps
+    its part in the gradient, - g p_j, as the formula has it."""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dtype not in DTYPES or logits.dim() < 1:
+        raise ValueError("logits must be a cuda float32, bfloat16 or float16 tensor [..., V]")
+    lead, v = logits.shape[:-1], logits.shape[-1]
+    if v < 1 or v > 1 << 30:
+        raise ValueError("logits must have 1 to 2^30 actions a row, got %d" % v)
+    if isinstance(top, bool) or not isinstance(top, int) or not 0 <= top <= MOST:
+        raise ValueError("top must be an int from 0 to %d" % MOST)
+    temperature = float(temperature)
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError("temperature must be positive and finite (1e-30 to 1e30), got %r" % temperature)
+    x = logits if logits.dim() == 2 else logits.reshape(-1, v)
+    if x.stride(1) != 1 and v > 1:
+        x = x.contiguous()
+    shape = None
+    if actions is not None:
+        if not isinstance(actions, torch.Tensor) or actions.device != logits.device or actions.dtype not in (torch.int64, torch.int32):
+            raise ValueError("actions must be an int64 or int32 tensor on %s" % logits.device)
+        shape = actions.shape
+        if shape != lead and (len(shape) != len(lead) + 1 or shape[:-1] != lead or not 1 <= shape[-1] <= MOST):
+            raise ValueError("actions must have the shape %s or %s + [1 .. %d], got %s" % (list(lead), list(lead), MOST, list(shape)))
+        actions = actions.reshape(x.shape[0], 1 if shape == lead else shape[-1]).contiguous()
+    mask_kind = MASK_NONE
+    if mask is not None:
+        mask, mask_kind = _check_mask(mask, lead, v, logits.device)
+    if x.requires_grad and torch.is_grad_enabled():
+        logp, entropy, top_action, top_logp = _Logprobs.apply(x, actions, mask, mask_kind, top, 1.0 / temperature)
+    else:
+        logp, entropy, top_action, top_logp, _ = _forward(x, actions, mask, mask_kind, top, 1.0 / temperature, False)
+    if len(lead) != 1:
+        entropy = entropy.reshape(lead)
+        if top:
+            top_action, top_logp = top_action.reshape(lead + (top,)), top_logp.reshape(lead + (top,))
+    if logp is not None and logp.shape != shape:
+        logp = logp.reshape(shape)
+    return ActionLogprobs(logp, entropy, top_action, top_logp)
+
+
+def legal_from_features(x):
+    """Network input [N, 8, 8, 14] -> bool [N, 512]: the legal actions its planes 6-13 hold (Checkers.py:431-432)."""
+    return (x[..., 6:14] != 0).permute(0, 3, 1, 2).reshape(x.shape[0], ACTIONS)
+
+
+@torch.no_grad()
+def rank_moves(net, boards, top=5, temperature=1.0):
+    """The moves that a network (net.PolicyValueNet, on the GPU, eval mode) considers in positions [N, 4] (rules.boards_to_device), best
+    first: RankedMoves(action int64 [N, top], logp [N, top], entropy [N], value [N]).  Probabilities are over the legal moves
+    (what `rules.mask_renorm` normalises to); action -1 where a position has fewer."""
+    mask, _ = rules.movegen(boards)
+    x = rules.features(boards).to(next(net.parameters()).dtype)
+    logits, value = net.logits(x.permute(0, 3, 1, 2))
+    out = action_logprobs(logits, mask=mask, top=top, temperature=temperature)
+    return RankedMoves(out.top_action, out.top_logp, out.entropy, value)

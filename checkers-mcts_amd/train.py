@@ -27,7 +27,7 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
-from . import _lib
+from . import _lib, policy
 from .net import PolicyValueNet
 
 TUPLE_BYTES = 288
@@ -228,21 +228,37 @@ def add_l2_gradients(net):
             torch._foreach_add_([t.grad for t in group], [t.detach() for t in group], alpha=2.0 * reg)
 
 
-def losses(net, x, pi, tv, autocast_dtype=None, with_penalty=True):
+def losses(net, x, pi, tv, autocast_dtype=None, with_penalty=True, entropy_weight=0.0):
     """(total, policy CE, value MSE) with Keras' definitions: CE = -sum(t * log(clip(p / sum p, 1e-7, 1 - 1e-7))).
     autocast_dtype (opt-in, TRAIN_DTYPE): run the convolutions / dense layers in that dtype (torch.autocast);
-    BatchNorm, softmax and the losses stay float32."""
+    BatchNorm, softmax and the losses stay float32.
+    entropy_weight (opt-in, ENTROPY_WEIGHT; GPU): the total loses entropy_weight x the mean entropy of the policy over the legal
+    actions (policy.action_logprobs), which keeps the policy from collapsing onto one move."""
+    z, run = None, net if not entropy_weight else net.logits
     if autocast_dtype is not None and autocast_dtype != torch.float32:
         with torch.autocast(device_type=x.device.type, dtype=autocast_dtype):
-            p, v = net(x.permute(0, 3, 1, 2))
+            p, v = run(x.permute(0, 3, 1, 2))
         p, v = p.float(), v.float()
     else:
-        p, v = net(x.permute(0, 3, 1, 2))
+        p, v = run(x.permute(0, 3, 1, 2))
+    if entropy_weight:
+        z, p = p, F.softmax(p, dim=1)
     p = p / p.sum(dim=1, keepdim=True)
     ce = -(pi * torch.log(p.clamp(1e-7, 1 - 1e-7))).sum(dim=1).mean()
     mse = F.mse_loss(v, tv)
     data_loss = net.policy_loss_weight * ce + net.value_loss_weight * mse
+    if entropy_weight:
+        data_loss = data_loss - entropy_weight * policy.action_logprobs(z, mask=policy.legal_from_features(x)).entropy.mean()
     return (data_loss + l2_penalty(net)) if with_penalty else data_loss, ce, mse
+
+
+@torch.no_grad()
+def policy_figures(net, x, pi):
+    """Sums over a batch (float64 [3]): the policy's entropy, the log probability of the most visited move, and how often that move is
+    among the network's three best -- all over the legal moves."""
+    move = pi.argmax(dim=1)
+    out = policy.action_logprobs(net.logits(x.permute(0, 3, 1, 2))[0], move, mask=policy.legal_from_features(x), top=3)
+    return torch.stack([out.entropy.double().sum(), out.logp.double().sum(), (out.top_action == move[:, None]).sum().double()])
 
 
 class History:
@@ -295,8 +311,26 @@ def train_nn(training_data, neural_network, **kwargs):
     clr = CyclicLR(base_lr=NN_BASE_LR, max_lr=NN_MAX_LR, step_size=int(CLR_SS_COEFF * (n_train / BATCH_SIZE)), mode="triangular")
     # the learning rate lives in a device tensor so that a captured step sees the cyclical schedule
     lr_t = torch.tensor(float(clr.on_train_begin()), dtype=torch.float32, device=dev)
-    opt = torch.optim.Adam(net.parameters(), lr=lr_t if dev.type == "cuda" else float(lr_t), betas=(0.9, 0.999), eps=1e-7,
-                           **({"fused": True, "capturable": True} if dev.type == "cuda" else {}))
+    # build-specific: OPTIMIZER "adam" (default, Keras' Adam) | "adamw" | "adamw8" (optim.AdamW, moments in 32 / 8 bits; WEIGHT_DECAY on the
+    # kernels of conv / dense layers, clipping at MAX_GRAD_NORM), ENTROPY_WEIGHT (losses()), POLICY_METRICS (validation figures)
+    optimizer, entropy_weight = kwargs.get("OPTIMIZER", "adam"), float(kwargs.get("ENTROPY_WEIGHT", 0.0))
+    policy_metrics = bool(kwargs.get("POLICY_METRICS", False))
+    if optimizer not in ("adam", "adamw", "adamw8"):
+        raise ValueError("OPTIMIZER must be 'adam', 'adamw' or 'adamw8'")
+    if optimizer == "adam" and ("WEIGHT_DECAY" in kwargs or "MAX_GRAD_NORM" in kwargs):
+        raise ValueError("WEIGHT_DECAY and MAX_GRAD_NORM belong to OPTIMIZER 'adamw' / 'adamw8'")
+    if dev.type != "cuda" and (optimizer != "adam" or entropy_weight or policy_metrics):
+        raise ValueError("OPTIMIZER 'adamw' / 'adamw8', ENTROPY_WEIGHT and POLICY_METRICS run on a GPU")
+    if optimizer == "adam":
+        opt = torch.optim.Adam(net.parameters(), lr=lr_t if dev.type == "cuda" else float(lr_t), betas=(0.9, 0.999), eps=1e-7,
+                               **({"fused": True, "capturable": True} if dev.type == "cuda" else {}))
+    else:
+        from .optim import AdamW
+        kernels = [m.weight for m in net.modules() if isinstance(m, (torch.nn.Conv2d, torch.nn.Linear))]
+        others = [p for p in net.parameters() if all(p is not k for k in kernels)]
+        opt = AdamW([{"params": kernels}, {"params": others, "weight_decay": 0.0}], lr=lr_t, betas=(0.9, 0.999), eps=1e-7,
+                    weight_decay=float(kwargs.get("WEIGHT_DECAY", 0.01)), state_bits=8 if optimizer == "adamw8" else 32,
+                    max_norm=kwargs.get("MAX_GRAD_NORM"), seed=int(kwargs.get("SEED", 0)))
     # ModelCheckpoint's file, training_pipeline.py:139-141 (MODEL_SUFFIX '.pt': a torch state_dict instead of Keras HDF5)
     filepath = "data/model/Checkers_Model" + str(TRAINING_ITERATION + 1) + "_" + create_timestamp() + kwargs.get("MODEL_SUFFIX", ".h5")
     os.makedirs("data/model", exist_ok=True)
@@ -310,11 +344,15 @@ def train_nn(training_data, neural_network, **kwargs):
     # epoch's last, ragged batch is filled up with randomly drawn training rows (see run()); "torch": autograd +
     # torch.optim.Adam (mixed-precision training, other network widths, and training sets smaller than one batch, which
     # the HIP step cannot fill)
+    # (OPTIMIZER "adamw" / "adamw8" and ENTROPY_WEIGHT are the autograd path's: the HIP step has Keras' loss and Adam built in)
+    chosen = "TRAIN_BACKEND" in kwargs or optimizer != "adam" or entropy_weight != 0.0
     backend = kwargs.get("TRAIN_BACKEND", "hip" if (dev.type == "cuda" and amp == torch.float32 and net.num_kernels == 128
-                                                     and BATCH_SIZE % 2 == 0) else "torch")
+                                                     and BATCH_SIZE % 2 == 0 and not chosen) else "torch")
+    if backend == "hip" and (optimizer != "adam" or entropy_weight):
+        raise ValueError("TRAIN_BACKEND 'hip' has Adam and no entropy term: OPTIMIZER 'adamw' / 'adamw8' and ENTROPY_WEIGHT need 'torch'")
     if backend == "hip" and n_train < BATCH_SIZE:
         backend = "torch"               # fewer rows than one batch: every step would take the torch path and leave the HIP weights untouched
-    if backend == "torch" and "TRAIN_BACKEND" not in kwargs and dev.type == "cuda":
+    if backend == "torch" and not chosen and dev.type == "cuda":
         import warnings                 # never a silent change of backend (as for inference: pipeline.EvaluatorPlan)
         warnings.warn("train_nn: the optimisation step runs on PyTorch autograd / MIOpen, not on the hand-written kernels of ckr_train.hip "
                       "(they take the 128-kernel network in float32, an even BATCH_SIZE and at least one full batch of rows); "
@@ -331,7 +369,7 @@ def train_nn(training_data, neural_network, **kwargs):
             hip.step(x, pi, tv, lr_t, acc, n_rows)
             return
         opt.zero_grad(set_to_none=False)
-        loss, ce, mse = losses(net, x, pi, tv, amp, with_penalty=False)
+        loss, ce, mse = losses(net, x, pi, tv, amp, with_penalty=False, entropy_weight=entropy_weight)
         loss.backward()
         pen = l2_penalty_value(net)
         add_l2_gradients(net)
@@ -364,6 +402,7 @@ def train_nn(training_data, neural_network, **kwargs):
         else:
             acc = torch.zeros(3, dtype=torch.float64, device=dev)
         pen_eval = None if train else l2_penalty_value(net)
+        figures = torch.zeros(3, dtype=torch.float64, device=dev)
         rows_seen = 0
         for b in batches:
             sel = idx[b * BATCH_SIZE:(b + 1) * BATCH_SIZE]
@@ -398,8 +437,13 @@ def train_nn(training_data, neural_network, **kwargs):
             else:
                 x, pi, tv = data.batch(sel)
                 with torch.no_grad():
-                    loss, ce, mse = losses(net, x, pi, tv, amp, with_penalty=False)
+                    loss, ce, mse = losses(net, x, pi, tv, amp, with_penalty=False, entropy_weight=entropy_weight)
+                    if policy_metrics:
+                        figures += policy_figures(net, x, pi)
                 acc += torch.stack([loss.detach() + pen_eval, ce.detach(), mse.detach()]).double() * float(sel.shape[0])
+        if not train and policy_metrics:
+            entropy, logp, top3 = (figures / float(rows_seen)).tolist()
+            history.add(val_policy_entropy=entropy, val_move_logp=logp, val_move_top3=top3)
         tot, ce_s, mse_s = (acc / float(rows_seen)).tolist()
         return tot, ce_s, mse_s
 

@@ -703,6 +703,72 @@ typedef struct {
 int ckr_adam_step(float* w, const float* grad, float* m, float* v, const float* reg, int64_t n, const float* d_lr, float beta1,
                   float beta2, float eps, float* d_step, double* d_penalty_parts, const ckr_loss_args* losses, void* stream);
 
+/* ---- log probabilities of given actions, entropy, top alternatives ------------------------------------------------ *
+ * The reference reads its policy as a dense masked softmax only (Checkers.predict, Checkers.py:425-438; nothing there asks
+ * for the probability of a given move, the policy's entropy or its best candidates); these have no counterpart in it.
+ * Row x of n rows of v logits (element (i, j) at logits[i * row_stride + j]; row_stride 0: every row the same), tau =
+ * 1 / inv_temperature, A = the mask's actions without logits of -inf:
+ *     log p_j = (x_j - max) / tau - ln S, S = sum_A exp((x_j - max) / tau)       -inf outside A
+ *     logp[i][k]   = log p of actions[i][k]; a negative action: 0; an action >= v: NaN
+ *     entropy[i]   = -sum_A p_j log p_j
+ *     top_action / top_logp[i][0 .. top): the largest of A, ties to the lower action; -1 / -inf where A has fewer
+ * Empty A: log p -inf, entropy 0.  NaN or +inf in A: the row's numbers are NaN and its alternatives -1.  What is masked may
+ * hold anything.  v <= 2^30; at most CKR_LOGPROBS_MOST given actions and alternatives a row; any alignment.
+ * Masks: bytes (mask[i * mask_stride + j] != 0) or the 8 legal-move words of ckr_movegen_batch (v = 512, mask_stride in words);
+ * mask_stride 0: one mask for all rows.
+ * stats (forward: may be NULL): what the backward pass needs of a row, 4 floats.
+ * Backward: grad[i * grad_stride + j] = dL/dx_j in the logits' type, from g_logp[n][n_given] and g_entropy[n] (NULL: 0); an
+ * action >= v makes the row's gradient NaN, a given action outside A keeps its part -g p_j.  scratch: ckr_logprobs_scratch
+ * bytes of device memory, of no content, for the duration of the call's kernels (0: may be NULL). */
+#define CKR_F32 0
+#define CKR_BF16 1
+#define CKR_F16 2
+#define CKR_MASK_NONE 0
+#define CKR_MASK_BYTES 1
+#define CKR_MASK_LEGAL 2
+#define CKR_LOGPROBS_MOST 64
+typedef struct {
+    const void* logits; const void* actions; const void* mask;
+    float* logp; float* entropy; int64_t* top_action; float* top_logp; float* stats;
+    const float* g_logp; const float* g_entropy; void* grad; void* scratch;
+    int64_t n, v, row_stride, mask_stride, grad_stride, scratch_bytes;
+    int32_t dtype, mask_kind, action_bytes, n_given, top;     /* action_bytes: 4 or 8 */
+    float inv_temperature;
+} ckr_logprobs_args;
+int64_t ckr_logprobs_scratch(const ckr_logprobs_args* a);     /* bytes for the forward pass of these sizes; negative: a ckr_status */
+int ckr_logprobs_forward(const ckr_logprobs_args* a, void* stream);
+int ckr_logprobs_backward(const ckr_logprobs_args* a, void* stream);
+
+/* ---- AdamW over many tensors ---------------------------------------------------------------------------------------- *
+ * Decoupled weight decay; the reference trains with Keras' Adam and l2 penalties (training_pipeline.py:49-114), which is
+ * ckr_adam_step.  count tensors of one type: sizes[i] elements at params[i] / grads[i] (host arrays of device pointers; a NULL
+ * gradient leaves its tensor, states and step number alone), states at element offsets[i] (a multiple of 128) of m, v and master,
+ * each tensor's part padded to whole blocks of 128.
+ *     g = c grad;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  t = ++d_step[i]
+ *     w = w (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+ * c = d_norm[1] (NULL: 1); lr = *d_lr, or lr where d_lr is NULL.  Parameters of 16 bits: w is the float32 master copy, the
+ * parameter its rounding.  state_bits 32: m, v float32.  state_bits 8: bytes with a scale byte for each 128 elements
+ * (m_scale, v_scale); m: sign, 4 exponent, 3 mantissa bits, v: 5 exponent, 3 mantissa bits, rounded stochastically with the bits of
+ * Philox4x32-10 (key seed, counter (element / 8, t)).  d_ticket: a word that is 0 before the first call and not shared with
+ * calls that may run at the same time. */
+typedef struct {
+    const int64_t* sizes; const int64_t* offsets; void* const* params; const void* const* grads;
+    float* master; void* m; void* v; uint8_t* m_scale; uint8_t* v_scale;
+    int32_t* d_step; uint32_t* d_ticket; const float* d_lr; const double* d_norm;
+    double lr, beta1, beta2, weight_decay; uint64_t seed;
+    float eps; int32_t count, dtype, state_bits;
+} ckr_adamw_args;
+int ckr_adamw_step(const ckr_adamw_args* a, void* stream);
+/* d_out[0] = sqrt of the sum of squares of all gradients (float64 sums in a fixed order), d_out[1] = min(1, max_norm / (d_out[0] +
+ * 1e-6)).  d_parts: room for `parts` partial sums, 2048 for each run of up to 96 tensors of one type is enough. */
+int ckr_grad_norm(int32_t count, const int64_t* sizes, const void* const* grads, const int32_t* dtypes, double max_norm, double* d_parts,
+                  int64_t parts, uint32_t* d_ticket, double* d_out, void* stream);
+/* 8-bit moments as float32 values, and float32 values as 8-bit moments (to the nearest code); n: a multiple of 128. */
+int ckr_adamw_read_moments(const uint8_t* m, const uint8_t* v, const uint8_t* m_scale, const uint8_t* v_scale, int64_t n, float* m_out,
+                           float* v_out, void* stream);
+int ckr_adamw_write_moments(const float* m_in, const float* v_in, int64_t n, uint8_t* m, uint8_t* v, uint8_t* m_scale, uint8_t* v_scale,
+                            void* stream);
+
 /* ---- probes of the stochastic paths (parity tests only) ------------------ *
  * The reference draws from NumPy's MT19937 (np.random.dirichlet, MCTS.py:107-108; np.random.choice,
  * MCTS.py:246), which cannot be reproduced bit for bit; the engine uses Philox4x32-10.  These entry
