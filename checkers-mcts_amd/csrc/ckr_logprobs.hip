@@ -17,7 +17,16 @@ constexpr float LOWEST = -3.402823466e38f, LOG2E = 1.44269504088896340736f;
 
 typedef ckr_logprobs_args Args;
 
-template <typename T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }
+constexpr float FLOOR = -1e30f;               // differences below it are that: exp is 0 anyway, and 0 x -inf would be NaN
+constexpr int PER_LANE = 32, TILE = 64 * PER_LANE;            // elements of a row that a wavefront holds in registers at a time
+
+// 16 bytes of logits that start at any element
+template <typename T> struct Vec {
+    static constexpr int N = 16 / sizeof(T);
+    typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+};
+typedef uint8_t bytes4 __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint8_t bytes8 __attribute__((ext_vector_type(8), aligned(1)));
 
 template <int MASK> __device__ __forceinline__ bool is_allowed(const Args& A, long long row, int j) {
     if constexpr (MASK == CKR_MASK_BYTES) return static_cast<const uint8_t*>(A.mask)[row * A.mask_stride + j] != 0;
@@ -29,119 +38,354 @@ template <int MASK> __device__ __forceinline__ bool is_allowed(const Args& A, lo
     return true;
 }
 
+// elements j .. j + N - 1 as float32, -inf where they are masked or not below `end`; whole: all of them are below it
+template <typename T, int MASK, bool WHOLE>
+__device__ __forceinline__ void load_vec(const Args& A, long long row, const T* x, int j, int end, float* out) {
+    constexpr int N = Vec<T>::N;
+    if (WHOLE || j + N <= end) {
+        const typename Vec<T>::type v = *reinterpret_cast<const typename Vec<T>::type*>(x + j);
+#pragma unroll
+        for (int e = 0; e < N; ++e) out[e] = (float)v[e];
+        if constexpr (MASK == CKR_MASK_BYTES) {
+            const uint8_t* m = static_cast<const uint8_t*>(A.mask) + row * A.mask_stride + j;
+            if constexpr (N == 8) {
+                const bytes8 b = *reinterpret_cast<const bytes8*>(m);
+#pragma unroll
+                for (int e = 0; e < N; ++e) out[e] = b[e] ? out[e] : -__builtin_huge_valf();
+            } else {
+                const bytes4 b = *reinterpret_cast<const bytes4*>(m);
+#pragma unroll
+                for (int e = 0; e < N; ++e) out[e] = b[e] ? out[e] : -__builtin_huge_valf();
+            }
+        }
+        if constexpr (MASK == CKR_MASK_LEGAL) {                                   // j is a multiple of N: one word, four bits of it
+            const uint32_t w = static_cast<const uint32_t*>(A.mask)[row * A.mask_stride + (j >> 6)] >> (4 * ((j >> 3) & 7));
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int y = (j & 7) + e;
+                out[e] = ((((j >> 3) ^ y) & 1) && ((w >> (y >> 1)) & 1u)) ? out[e] : -__builtin_huge_valf();
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) out[e] = j + e < end && is_allowed<MASK>(A, row, j + e) ? (float)x[j + e] : -__builtin_huge_valf();
+    }
+}
+
 __device__ __forceinline__ long long action_at(const Args& A, long long i) {
     return A.action_bytes == 8 ? static_cast<const long long*>(A.actions)[i] : (long long)static_cast<const int*>(A.actions)[i];
 }
 
 __device__ __forceinline__ float wave_max_f32(float v) {
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+    v = fmaxf(v, bfly_f32<1>(v)); v = fmaxf(v, bfly_f32<2>(v)); v = fmaxf(v, bfly_f32<4>(v)); v = fmaxf(v, bfly_f32<8>(v));
+    const int i = __float_as_int(v);
+    return fmaxf(fmaxf(__int_as_float(__builtin_amdgcn_readlane(i, 0)), __int_as_float(__builtin_amdgcn_readlane(i, 16))),
+                 fmaxf(__int_as_float(__builtin_amdgcn_readlane(i, 32)), __int_as_float(__builtin_amdgcn_readlane(i, 48))));
 }
 __device__ __forceinline__ float wave_sum_f32(float v) {
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    v += bfly_f32<1>(v); v += bfly_f32<2>(v); v += bfly_f32<4>(v); v += bfly_f32<8>(v);
+    const int i = __float_as_int(v);
+    return (__int_as_float(__builtin_amdgcn_readlane(i, 0)) + __int_as_float(__builtin_amdgcn_readlane(i, 16))) +
+           (__int_as_float(__builtin_amdgcn_readlane(i, 32)) + __int_as_float(__builtin_amdgcn_readlane(i, 48)));
+}
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }          // 1 ulp; denormal results are 0
+
+// ---- a wavefront's k best (value, index) so far: lane r holds the one of rank r; larger value first, then lower index --------------
+struct TopList {
+    float v = -__builtin_huge_valf();
+    int i = -1;
+    // what a candidate has to beat: the entry of rank k - 1, or (an element has to equal it at least) a bound from below
+    float tau = -__builtin_huge_valf();
+    int tau_i = -1;
+
+    __device__ __forceinline__ void insert(float x, int j, int k) {               // x, j: the same in all lanes
+        const int pos = __popcll(__ballot(v > x || (v == x && i < j)));
+        const float vs = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x138, 0xF, 0xF, false));      // wave_shr:1
+        const int is = __builtin_amdgcn_update_dpp(0, i, 0x138, 0xF, 0xF, false);
+        const int lane = lane_id();
+        v = lane < pos ? v : lane == pos ? x : vs;
+        i = lane < pos ? i : lane == pos ? j : is;
+        const float kv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), k - 1));
+        if (kv > -__builtin_huge_valf()) { tau = kv; tau_i = __builtin_amdgcn_readlane(i, k - 1); }
+    }
+    // every lane's candidate (x, j); -inf and NaN are none
+    __device__ __forceinline__ void offer(float x, int j, int k) {
+        unsigned long long m = __ballot(x > tau || (x == tau && j < tau_i));
+        while (m) {
+            const int l = first_lane(m);
+            m &= m - 1;
+            const float xl = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l));
+            const int jl = __builtin_amdgcn_readlane(j, l);
+            if (xl > tau || (xl == tau && jl < tau_i)) insert(xl, jl, k);
+        }
+    }
+    // While the list is not full: k of the lanes have a candidate >= the k-th largest of their maxima `t`, so what is below it is none.
+    __device__ __forceinline__ void bound_from_below(float t, int k) {
+        float x = -__builtin_huge_valf();
+        for (int r = 0; r < k; ++r) {
+            x = wave_max_f32(t);
+            if (!(x > -__builtin_huge_valf())) return;
+            const int l = first_lane(__ballot(t == x));
+            t = lane_id() == l ? -__builtin_huge_valf() : t;
+        }
+        tau = x; tau_i = 0x7FFFFFFF;
+    }
+};
+
+// ---- forward: what a wavefront knows of its part of a row --------------------------------------------------------------------------
+// m: the maximum, S = sum exp(it (x - m)), D = sum exp(it (x - m)) (x - m), per lane until they are joined.  One pass: where a tile raises a
+// lane's maximum, its sums are carried over to the new one, S' = f S, D' = f (D + (m - m') S) with f = exp(it (m - m')).
+struct Sums { float m, S, D; };
+
+__device__ __forceinline__ void carry(Sums& s, float m, float c) {
+    const float d = fmaxf(s.m - m, FLOOR), f = exp2_fast(d * c);
+    s.D = f * __builtin_fmaf(d, s.S, s.D);
+    s.S *= f;
+    s.m = m;
 }
 
-// One wavefront per row: the maximum, then the sums, then every alternative by a pass of its own (the largest element behind the
-// last one in the order "larger value, lower index").
-template <typename T, int MASK>
-__global__ __launch_bounds__(256) void k_logprobs(const Args A) {
-    const int lane = lane_id(), V = (int)A.v;
-  for (long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); row < A.n; row += 4ll * gridDim.x) {
+template <typename T, int MASK, bool TOP>
+__device__ __forceinline__ void scan(const Args& A, long long row, int begin, int end, Sums& s, TopList& list) {
+    constexpr int N = Vec<T>::N, U = PER_LANE / N;
     const T* x = static_cast<const T*>(A.logits) + row * A.row_stride;
-    const float it = A.inv_temperature;
-    float m = LOWEST;
-    for (int j = lane; j < V; j += 64)
-        if (is_allowed<MASK>(A, row, j)) m = fmaxf(m, to_f32(x[j]));
-    m = wave_max_f32(m);
-    float S = 0.0f, D = 0.0f;
-    for (int j = lane; j < V; j += 64)
-        if (is_allowed<MASK>(A, row, j)) {
-            const float d = to_f32(x[j]) - m, e = exp2f(d * (it * LOG2E));
-            S += e;
-            D += e > 0.0f ? e * d : 0.0f;
+    const int lane = lane_id(), k = A.top;
+    const float c = A.inv_temperature * LOG2E;
+    s.m = LOWEST; s.S = 0.0f; s.D = 0.0f;
+    for (int j0 = begin; j0 < end; j0 += TILE) {
+        float v[PER_LANE], vm[U], tm = -__builtin_huge_valf();
+        const int left = (end - j0 + 64 * N - 1) / (64 * N);                      // vectors of this tile that hold anything
+        if (j0 + TILE <= end) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) load_vec<T, MASK, true>(A, row, x, j0 + (u * 64 + lane) * N, end, v + u * N);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (u < left) load_vec<T, MASK, false>(A, row, x, j0 + (u * 64 + lane) * N, end, v + u * N);
         }
-    S = wave_sum_f32(S); D = wave_sum_f32(D);
-    const bool empty = S == 0.0f, bad = !(S < __builtin_huge_valf());
-    const float lnS = empty ? 0.0f : logf(S), H = empty ? 0.0f : lnS - it * D / S;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            vm[u] = -__builtin_huge_valf();
+            if (u < left) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) vm[u] = fmaxf(vm[u], v[u * N + e]);
+            }
+            tm = fmaxf(tm, vm[u]);
+        }
+        if (__any(tm > s.m)) carry(s, fmaxf(tm, s.m), c);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (u < left) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const float d = v[u * N + e] - s.m, p = exp2_fast(d * c);
+                    s.S += p;
+                    s.D = __builtin_fmaf(p, fmaxf(d, FLOOR), s.D);
+                }
+            }
+        if constexpr (TOP) {
+            if (!(list.tau > -__builtin_huge_valf())) list.bound_from_below(tm, k);
+            // elements come in rising vectors: one that equals the last entry of an earlier vector comes behind it
+            if (__any(list.tau_i < j0 ? tm > list.tau : tm >= list.tau)) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (u < left && __any(vm[u] >= list.tau)) {
+#pragma unroll
+                        for (int e = 0; e < N; ++e) list.offer(v[u * N + e], j0 + (u * 64 + lane) * N + e, k);
+                    }
+            }
+        }
+    }
+}
+
+// the lanes' sums over one maximum
+__device__ __forceinline__ void join_lanes(Sums& s, float c) {
+    carry(s, wave_max_f32(s.m), c);
+    s.S = wave_sum_f32(s.S); s.D = wave_sum_f32(s.D);
+}
+
+template <typename T, int MASK, bool TOP>
+__device__ __forceinline__ void write_row(const Args& A, long long row, const Sums& s, const TopList& list) {
+    const int lane = lane_id();
+    const float it = A.inv_temperature;
+    const bool empty = s.S == 0.0f, bad = !(s.S < __builtin_huge_valf());
+    const float lnS = empty ? 0.0f : logf(s.S), H = empty ? 0.0f : lnS - it * s.D / s.S;
     if (lane == 0) {
         A.entropy[row] = H;
-        if (A.stats) { float* st = A.stats + 4 * row; st[0] = m; st[1] = S; st[2] = H; st[3] = 0.0f; }
+        if (A.stats) *reinterpret_cast<float4*>(A.stats + 4 * row) = make_float4(s.m, s.S, H, 0.0f);
     }
-    for (int k = lane; k < A.n_given; k += 64) {
-        const long long a = action_at(A, row * A.n_given + k);
+    if (lane < A.n_given) {
+        const long long a = action_at(A, row * A.n_given + lane);
+        const T* x = static_cast<const T*>(A.logits) + row * A.row_stride;
         float lp;
         if (a < 0) lp = 0.0f;
-        else if (a >= V || bad) lp = __builtin_nanf("");
-        else lp = !empty && is_allowed<MASK>(A, row, (int)a) ? (to_f32(x[a]) - m) * it - lnS : -__builtin_huge_valf();
-        A.logp[row * A.n_given + k] = lp;
+        else if (a >= A.v || bad) lp = __builtin_nanf("");
+        else lp = !empty && is_allowed<MASK>(A, row, (int)a) ? ((float)x[a] - s.m) * it - lnS : -__builtin_huge_valf();
+        A.logp[row * A.n_given + lane] = lp;
     }
-    float last = __builtin_huge_valf();
-    int last_j = -1;
-    for (int k = 0; k < A.top; ++k) {
-        float best = -__builtin_huge_valf();
-        int best_j = -1;
-        if (!bad)
-            for (int j = lane; j < V; j += 64)
-                if (is_allowed<MASK>(A, row, j)) {
-                    const float v = to_f32(x[j]);
-                    if ((v < last || (v == last && j > last_j)) && v > best) { best = v; best_j = j; }
-                }
-        const float top = wave_max_f32(best);
-        int j = best_j >= 0 && best == top ? best_j : 0x7FFFFFFF;
-        for (int o = 32; o; o >>= 1) j = min(j, __shfl_xor(j, o));
-        const bool none = j == 0x7FFFFFFF;
-        if (lane == 0) {
-            A.top_action[row * A.top + k] = none ? -1 : j;
-            A.top_logp[row * A.top + k] = bad ? __builtin_nanf("") : none ? -__builtin_huge_valf() : (top - m) * it - lnS;
-        }
-        last = none ? -__builtin_huge_valf() : top; last_j = none ? V : j;
+    if (TOP && lane < A.top) {
+        A.top_action[row * A.top + lane] = bad ? -1 : list.i;
+        A.top_logp[row * A.top + lane] = bad ? __builtin_nanf("") : list.i < 0 ? -__builtin_huge_valf() : (list.v - s.m) * it - lnS;
     }
-  }
 }
+
+// parts == 1: a wavefront per row.  Otherwise the row is cut into `parts` of `length` elements (whole tiles), a wavefront each, whose sums
+// and lists go to the scratch memory for k_logprobs_join: float4 [rows][parts], values and indexes [rows][parts][top].
+template <typename T, int MASK, bool TOP>
+__global__ __launch_bounds__(256) void k_logprobs(const Args A, int parts, int length) {
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    Sums s;
+    if (parts == 1) {
+        for (long long row = (long long)blockIdx.x * 4 + wave; row < A.n; row += 4ll * gridDim.x) {
+            TopList list;
+            scan<T, MASK, TOP>(A, row, 0, (int)A.v, s, list);
+            join_lanes(s, A.inv_temperature * LOG2E);
+            write_row<T, MASK, TOP>(A, row, s, list);
+        }
+        return;
+    }
+    const int part = (int)blockIdx.x * 4 + wave;
+    if (part >= parts) return;
+    const int begin = part * length, end = (int)A.v - begin < length ? (int)A.v : begin + length;
+    for (long long row = blockIdx.y; row < A.n; row += gridDim.y) {
+        TopList list;
+        scan<T, MASK, TOP>(A, row, begin, end, s, list);
+        join_lanes(s, A.inv_temperature * LOG2E);
+        const long long at = row * parts + part;
+        float4* sums = static_cast<float4*>(A.scratch);
+        if (lane_id() == 0) sums[at] = make_float4(s.m, s.S, s.D, 0.0f);
+        if (TOP && lane_id() < A.top) {
+            float* tv = reinterpret_cast<float*>(sums + A.n * parts);
+            int* ti = reinterpret_cast<int*>(tv + A.n * parts * A.top);
+            tv[at * A.top + lane_id()] = list.v;
+            ti[at * A.top + lane_id()] = list.i;
+        }
+    }
+}
+
+template <typename T, int MASK, bool TOP>
+__global__ __launch_bounds__(64) void k_logprobs_join(const Args A, int parts) {
+    const int lane = lane_id();
+    const float c = A.inv_temperature * LOG2E;
+    const float4* sums = static_cast<const float4*>(A.scratch);
+    const float* tv = reinterpret_cast<const float*>(sums + A.n * parts);
+    const int* ti = reinterpret_cast<const int*>(tv + A.n * parts * A.top);
+    for (long long row = blockIdx.x; row < A.n; row += gridDim.x) {
+        Sums s = {LOWEST, 0.0f, 0.0f};
+        for (int p = lane; p < parts; p += 64) {
+            const float4 o = sums[row * parts + p];
+            Sums t = {o.x, o.y, o.z};
+            const float m = fmaxf(s.m, t.m);
+            carry(s, m, c);
+            carry(t, m, c);
+            s.S += t.S; s.D += t.D;
+        }
+        join_lanes(s, c);
+        TopList list;
+        if constexpr (TOP) {
+            const int n = parts * A.top;
+            for (int q = 0; q < n; q += 64) {
+                const bool have = q + lane < n;
+                const float x = have ? tv[row * n + q + lane] : -__builtin_huge_valf();
+                if (!(list.tau > -__builtin_huge_valf())) list.bound_from_below(x, A.top);
+                list.offer(x, have ? ti[row * n + q + lane] : -1, A.top);
+            }
+        }
+        write_row<T, MASK, TOP>(A, row, s, list);
+    }
+}
+
+// ---- backward: a wavefront has BWD_PER_LANE elements a lane of one row ----------------------------------------------------------------
+constexpr int BWD_PER_LANE = 16, BWD_TILE = 64 * BWD_PER_LANE;
 
 template <typename T, int MASK>
 __global__ __launch_bounds__(256) void k_logprobs_bwd(const Args A) {
-    const int V = (int)A.v;
-    const float it = A.inv_temperature;
-    for (long long row = blockIdx.x; row < A.n; row += gridDim.x) {
-        const float* st = A.stats + 4 * row;
-        const float m = st[0], S = st[1], H = st[2], h = A.g_entropy ? A.g_entropy[row] : 0.0f;
-        const float lnS = logf(S);
+    constexpr int N = Vec<T>::N, U = BWD_PER_LANE / N;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), V = (int)A.v;
+    const int j0 = ((int)blockIdx.x * 4 + wave) * BWD_TILE;
+    if (j0 >= V) return;
+    const float it = A.inv_temperature, c = it * LOG2E;
+    for (long long row = blockIdx.y; row < A.n; row += gridDim.y) {
         const T* x = static_cast<const T*>(A.logits) + row * A.row_stride;
         T* out = static_cast<T*>(A.grad) + row * A.grad_stride;
-        float G = 0.0f;
-        for (int k = 0; k < A.n_given; ++k) {
-            const long long a = action_at(A, row * A.n_given + k);
-            if (a >= V) G = __builtin_nanf("");
-            else if (a >= 0) G += A.g_logp[row * A.n_given + k];
+        float v[BWD_PER_LANE], given[BWD_PER_LANE];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = j0 + (u * 64 + lane) * N;
+            if (j0 + BWD_TILE <= V) load_vec<T, MASK, true>(A, row, x, j, V, v + u * N);
+            else load_vec<T, MASK, false>(A, row, x, j, V, v + u * N);
         }
-        for (int j = threadIdx.x; j < V; j += 256) {
-            const float v = to_f32(x[j]);
-            float dx = 0.0f;
-            if (is_allowed<MASK>(A, row, j) && v != -__builtin_huge_valf()) {
-                const float d = v - m, p = exp2f(d * (it * LOG2E)) / S;
-                float given = 0.0f;
-                for (int k = 0; k < A.n_given; ++k)
-                    if (action_at(A, row * A.n_given + k) == j) given += A.g_logp[row * A.n_given + k];
-                const float c = p > 0.0f ? G + h * ((d * it - lnS) + H) : p * G;
-                dx = it * (given - p * c);
+        const float4 st = *reinterpret_cast<const float4*>(A.stats + 4 * row);
+        const float m = st.x, rS = 1.0f / st.y, lnS = logf(st.y), H = st.z, h = A.g_entropy ? A.g_entropy[row] : 0.0f;
+        // lane k has the k-th given action; those of this tile go to the lanes that hold their elements, in the order of k
+        long long a = -1;
+        float g = 0.0f;
+        if (lane < A.n_given) {
+            a = action_at(A, row * A.n_given + lane);
+            g = a < 0 ? 0.0f : a >= V ? __builtin_nanf("") : A.g_logp[row * A.n_given + lane];
+        }
+        const float G = wave_sum_f32(g);
+#pragma unroll
+        for (int e = 0; e < BWD_PER_LANE; ++e) given[e] = 0.0f;
+        for (unsigned long long mine = __ballot(a >= j0 && a < (long long)j0 + BWD_TILE && a < V); mine; mine &= mine - 1) {
+            const int l = first_lane(mine);
+            const int off = __builtin_amdgcn_readlane((int)a, l) - j0 - lane * N;
+            const float gl = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), l));
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < N; ++e) given[u * N + e] += off == u * 64 * N + e ? gl : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            typename Vec<T>::type r;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float x1 = v[u * N + e], d = x1 - m, p = exp2_fast(d * c) * rS;
+                const float lp = fmaxf(__builtin_fmaf(d, it, -lnS), -200.0f);         // p is 0 below -104: any finite number does
+                const float q = p * __builtin_fmaf(h, lp + H, G);
+                r[e] = (T)(x1 == -__builtin_huge_valf() ? 0.0f : it * (given[u * N + e] - q));
             }
-            out[j] = (T)dx;
+            const int j = j0 + (u * 64 + lane) * N;
+            if (j + N <= V) *reinterpret_cast<typename Vec<T>::type*>(out + j) = r;
+            else
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (j + e < V) out[j + e] = r[e];
         }
     }
 }
 
-template <typename T> int forward_t(const Args& A, hipStream_t s) {
-    const dim3 grid((unsigned)(A.n < (1 << 22) ? (A.n + 3) / 4 : 1 << 20)), block(256);
-    if (A.mask_kind == CKR_MASK_NONE) hipLaunchKernelGGL((k_logprobs<T, CKR_MASK_NONE>), grid, block, 0, s, A);
-    else if (A.mask_kind == CKR_MASK_BYTES) hipLaunchKernelGGL((k_logprobs<T, CKR_MASK_BYTES>), grid, block, 0, s, A);
-    else hipLaunchKernelGGL((k_logprobs<T, CKR_MASK_LEGAL>), grid, block, 0, s, A);
+// How many parts a row is cut into.  A wavefront per row fills the card from about WAVES rows on; below that a row's tiles are spread over
+// more wavefronts, and a second launch joins them.
+constexpr int WAVES = 4096;
+static void split(const Args& A, int& parts, int& length) {
+    const long long tiles = (A.v + TILE - 1) / TILE;
+    const long long want = A.n >= WAVES / 2 ? 1 : (WAVES + A.n - 1) / (A.n > 0 ? A.n : 1);
+    const long long each = tiles <= want ? 1 : (tiles + want - 1) / want;         // tiles of a part
+    parts = (int)((tiles + each - 1) / each);
+    length = parts == 1 ? (int)A.v : (int)each * TILE;
+}
+
+template <typename T, int MASK, bool TOP> int forward_tmk(const Args& A, hipStream_t s) {
+    int parts, length;
+    split(A, parts, length);
+    const long long rows4 = (A.n + 3) / 4;
+    const dim3 grid = parts == 1 ? dim3((unsigned)(rows4 < (1 << 20) ? rows4 : 1 << 20)) : dim3((unsigned)((parts + 3) / 4), (unsigned)(A.n < 65535 ? A.n : 65535));
+    hipLaunchKernelGGL((k_logprobs<T, MASK, TOP>), grid, dim3(256), 0, s, A, parts, length);
     CKR_HIP(hipGetLastError());
+    if (parts > 1) {
+        hipLaunchKernelGGL((k_logprobs_join<T, MASK, TOP>), dim3((unsigned)(A.n < (1 << 20) ? A.n : 1 << 20)), dim3(64), 0, s, A, parts);
+        CKR_HIP(hipGetLastError());
+    }
     return CKR_OK;
 }
+template <typename T> int forward_t(const Args& A, hipStream_t s) {
+    if (A.mask_kind == CKR_MASK_NONE) return A.top ? forward_tmk<T, CKR_MASK_NONE, true>(A, s) : forward_tmk<T, CKR_MASK_NONE, false>(A, s);
+    if (A.mask_kind == CKR_MASK_BYTES) return A.top ? forward_tmk<T, CKR_MASK_BYTES, true>(A, s) : forward_tmk<T, CKR_MASK_BYTES, false>(A, s);
+    return A.top ? forward_tmk<T, CKR_MASK_LEGAL, true>(A, s) : forward_tmk<T, CKR_MASK_LEGAL, false>(A, s);
+}
 template <typename T> int backward_t(const Args& A, hipStream_t s) {
-    const dim3 grid((unsigned)(A.n < (1 << 20) ? A.n : 1 << 20)), block(256);
+    const dim3 grid((unsigned)((A.v + 4 * BWD_TILE - 1) / (4 * BWD_TILE)), (unsigned)(A.n < 65535 ? A.n : 65535)), block(256);
     if (A.mask_kind == CKR_MASK_NONE) hipLaunchKernelGGL((k_logprobs_bwd<T, CKR_MASK_NONE>), grid, block, 0, s, A);
     else if (A.mask_kind == CKR_MASK_BYTES) hipLaunchKernelGGL((k_logprobs_bwd<T, CKR_MASK_BYTES>), grid, block, 0, s, A);
     else hipLaunchKernelGGL((k_logprobs_bwd<T, CKR_MASK_LEGAL>), grid, block, 0, s, A);
@@ -159,7 +403,8 @@ static int check_args(const Args* a, const char* who) {
     if (a->n_given < 0 || a->n_given > CKR_LOGPROBS_MOST || a->top < 0 || a->top > CKR_LOGPROBS_MOST)
         return fail(CKR_ERR_INVALID, "%s: at most %d given actions and alternatives a row", who, CKR_LOGPROBS_MOST);
     if (a->n && a->n_given && (!a->actions || (a->action_bytes != 4 && a->action_bytes != 8))) return fail(CKR_ERR_INVALID, "%s: bad actions", who);
-    if (!(a->inv_temperature > 0.0f) || !(a->inv_temperature < __builtin_huge_valf())) return fail(CKR_ERR_INVALID, "%s: the temperature must be positive and finite", who);
+    if (!(a->inv_temperature >= 9.9e-7f && a->inv_temperature <= 1.01e6f)) return fail(CKR_ERR_INVALID, "%s: the temperature must be from 1e-6 to 1e6", who);
+    if ((reinterpret_cast<uintptr_t>(a->stats) | reinterpret_cast<uintptr_t>(a->scratch)) & 15) return fail(CKR_ERR_INVALID, "%s: stats and scratch begin at multiples of 16 bytes", who);
     if (a->row_stride < 0 || (a->n && !a->logits)) return fail(CKR_ERR_INVALID, "%s: bad logits", who);
     return CKR_OK;
 }
@@ -170,13 +415,17 @@ extern "C" {
 
 int64_t ckr_logprobs_scratch(const ckr_logprobs_args* a) {
     if (int rc = ckr::check_args(a, "ckr_logprobs_scratch")) return rc;
-    return 0;
+    int parts, length;
+    ckr::split(*a, parts, length);
+    return parts == 1 ? 0 : a->n * parts * (16 + 8 * (int64_t)a->top);
 }
 
 int ckr_logprobs_forward(const ckr_logprobs_args* a, void* stream) {
     if (int rc = ckr::check_args(a, "ckr_logprobs_forward")) return rc;
     if (a->n && (!a->entropy || (a->n_given && !a->logp) || (a->top && (!a->top_action || !a->top_logp))))
         return ckr::fail(CKR_ERR_INVALID, "ckr_logprobs_forward: null output");
+    const int64_t scratch = ckr_logprobs_scratch(a);
+    if (scratch > 0 && (!a->scratch || a->scratch_bytes < scratch)) return ckr::fail(CKR_ERR_INVALID, "ckr_logprobs_forward: %lld bytes of scratch memory needed", (long long)scratch);
     if (int rc = ckr::require_device()) return rc;
     if (!a->n) return CKR_OK;
     if (a->dtype == CKR_F32) return ckr::forward_t<float>(*a, (hipStream_t)stream);

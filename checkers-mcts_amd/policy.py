@@ -131,6 +131,7 @@ def action_logprobs(logits, actions=None, mask=None, top=0, temperature=1.0):
               gradient); one >= V gives NaN, and a NaN gradient in its row.
     mask      the actions that count: bool [..., V], [V] or broadcastable (True: allowed), or the int32 [..., 8] legal-move words of
               `rules.movegen` (V = 512).  A logit of -inf is masked too; what is masked may hold anything, NaN included.
+    temperature  1e-6 to 1e6.
     top       up to 64 alternatives: the most likely allowed actions, ties to the lower action.
 
     Returns ActionLogprobs(logp, entropy, top_action, top_logp), float32 and int64 (None for what was not asked).  A masked action has log p
@@ -147,8 +148,8 @@ def action_logprobs(logits, actions=None, mask=None, top=0, temperature=1.0):
     if isinstance(top, bool) or not isinstance(top, int) or not 0 <= top <= MOST:
         raise ValueError("top must be an int from 0 to %d" % MOST)
     temperature = float(temperature)
-    if not 1e-30 <= temperature <= 1e30:
-        raise ValueError("temperature must be positive and finite (1e-30 to 1e30), got %r" % temperature)
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError("temperature must be from 1e-6 to 1e6, got %r" % temperature)
     x = logits if logits.dim() == 2 else logits.reshape(-1, v)
     if x.stride(1) != 1 and v > 1:
         x = x.contiguous()

@@ -713,7 +713,8 @@ int ckr_adam_step(float* w, const float* grad, float* m, float* v, const float* 
  *     entropy[i]   = -sum_A p_j log p_j
  *     top_action / top_logp[i][0 .. top): the largest of A, ties to the lower action; -1 / -inf where A has fewer
  * Empty A: log p -inf, entropy 0.  NaN or +inf in A: the row's numbers are NaN and its alternatives -1.  What is masked may
- * hold anything.  v <= 2^30; at most CKR_LOGPROBS_MOST given actions and alternatives a row; any alignment.
+ * hold anything.  v <= 2^30; tau from 1e-6 to 1e6; at most CKR_LOGPROBS_MOST given actions and alternatives a row; logits, masks and
+ * gradients of any alignment, stats and scratch of 16 bytes.
  * Masks: bytes (mask[i * mask_stride + j] != 0) or the 8 legal-move words of ckr_movegen_batch (v = 512, mask_stride in words);
  * mask_stride 0: one mask for all rows.
  * stats (forward: may be NULL): what the backward pass needs of a row, 4 floats.
