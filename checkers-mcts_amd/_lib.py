@@ -146,6 +146,13 @@ def load():
     return L
 
 
+def raw_stream(device_index):
+    """hipStream_t of a device's current stream, as an integer."""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)         # what current_stream().cuda_stream returns, without a Stream object
+    return raw(device_index) if raw is not None else torch.cuda.current_stream(device_index).cuda_stream
+
+
 def check(rc):
     if rc != 0:
         msg = load().ckr_last_error().decode("utf-8", "replace")

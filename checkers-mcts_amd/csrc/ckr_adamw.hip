@@ -5,8 +5,8 @@
 //     w = w (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 // Parameters of 16 bits have a float32 master copy w; the parameter is its rounding.
 //
-// 8-bit moments: blocks of 128 elements, each with a scale byte b (the power of two 2^(b - 127), one above the block's largest value;
-// 255: the block holds a value that is not finite and reads back as NaN).  A code is a small float below that scale,
+// 8-bit moments: blocks of 128 elements, each with a scale byte b (2^(b - 127): the power of two of the block's largest value, or the
+// next one; 255: the block holds a value that is not finite and reads back as NaN).  A code is a small float below that scale,
 //     m: sign, 4 exponent bits, 3 mantissa bits   value (1 + M / 8) 2^(E - 15) 2^(b - 127)
 //     v: 5 exponent bits, 3 mantissa bits         value (1 + M / 8) 2^(E - 31) 2^(b - 127)
 // code 0 is 0.  A value of v below the smallest code is raised to it: as 0 it would divide by eps alone.
@@ -58,9 +58,10 @@ __device__ __forceinline__ int tensor_of(const TensorTable& T, unsigned c) {
 // ---- the 8-bit formats, on the high word of a double: 11 exponent bits, the first 20 bits of the mantissa ---------------------------
 __device__ __forceinline__ unsigned high_word(double x) { return (unsigned)__double2hiint(x) & 0x7FFFFFFFu; }
 
-// the scale byte of a block whose largest high word is h
-__device__ __forceinline__ int scale_byte(unsigned h) {
-    const int b = (int)(h >> 20) - 1023 + 1 + 127;
+// The scale byte of a block whose largest high word is h: one power above it (room = 1), so that a dithered rounding upwards stays in range;
+// from already rounded values (room = 0), the power they need, so that what codes hold is written back as it is.
+__device__ __forceinline__ int scale_byte(unsigned h, int room = 1) {
+    const int b = (int)(h >> 20) - 1023 + room + 127;
     return b > 254 ? 255 : b < 1 ? 1 : b;
 }
 template <int TOP> __device__ __forceinline__ int encode(unsigned h, int scale, unsigned dither17) {      // magnitude only, <= 0: below the smallest code
@@ -231,7 +232,7 @@ __global__ __launch_bounds__(256) void k_moments_write(const float* __restrict__
         unsigned hm = 0, hv = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) { hm = max(hm, high_word((double)m_in[i + j])); hv = max(hv, high_word((double)v_in[i + j])); }
-        const int ms = scale_byte(row16_max(hm)), vs = scale_byte(row16_max(hv));
+        const int ms = scale_byte(row16_max(hm) + 0x10000u, 0), vs = scale_byte(row16_max(hv) + 0x10000u, 0);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {                                             // to nearest: half a step is 2^16 of 2^17
             m[i + j] = (uint8_t)encode_m((double)m_in[i + j], ms, 0x10000u);

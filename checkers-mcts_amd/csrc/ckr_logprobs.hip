@@ -25,8 +25,6 @@ template <typename T> struct Vec {
     static constexpr int N = 16 / sizeof(T);
     typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
-typedef uint8_t bytes4 __attribute__((ext_vector_type(4), aligned(1)));
-typedef uint8_t bytes8 __attribute__((ext_vector_type(8), aligned(1)));
 
 template <int MASK> __device__ __forceinline__ bool is_allowed(const Args& A, long long row, int j) {
     if constexpr (MASK == CKR_MASK_BYTES) return static_cast<const uint8_t*>(A.mask)[row * A.mask_stride + j] != 0;
@@ -38,25 +36,18 @@ template <int MASK> __device__ __forceinline__ bool is_allowed(const Args& A, lo
     return true;
 }
 
-// elements j .. j + N - 1 as float32, -inf where they are masked or not below `end`; whole: all of them are below it
-template <typename T, int MASK, bool WHOLE>
-__device__ __forceinline__ void load_vec(const Args& A, long long row, const T* x, int j, int end, float* out) {
+// elements j .. j + N - 1 as float32, -inf where they are masked or not below `end`; `raw`: their logits, if all are below it
+template <typename T, int MASK>
+__device__ __forceinline__ void values(const Args& A, long long row, const T* x, int j, int end, const typename Vec<T>::type raw, float* out) {
     constexpr int N = Vec<T>::N;
-    if (WHOLE || j + N <= end) {
-        const typename Vec<T>::type v = *reinterpret_cast<const typename Vec<T>::type*>(x + j);
+    if (j + N <= end) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) out[e] = (float)v[e];
+        for (int e = 0; e < N; ++e) out[e] = (float)raw[e];
         if constexpr (MASK == CKR_MASK_BYTES) {
-            const uint8_t* m = static_cast<const uint8_t*>(A.mask) + row * A.mask_stride + j;
-            if constexpr (N == 8) {
-                const bytes8 b = *reinterpret_cast<const bytes8*>(m);
+            typedef uint8_t bytes __attribute__((ext_vector_type(N), aligned(1)));
+            const bytes m = *reinterpret_cast<const bytes*>(static_cast<const uint8_t*>(A.mask) + row * A.mask_stride + j);
 #pragma unroll
-                for (int e = 0; e < N; ++e) out[e] = b[e] ? out[e] : -__builtin_huge_valf();
-            } else {
-                const bytes4 b = *reinterpret_cast<const bytes4*>(m);
-#pragma unroll
-                for (int e = 0; e < N; ++e) out[e] = b[e] ? out[e] : -__builtin_huge_valf();
-            }
+            for (int e = 0; e < N; ++e) out[e] = m[e] ? out[e] : -__builtin_huge_valf();
         }
         if constexpr (MASK == CKR_MASK_LEGAL) {                                   // j is a multiple of N: one word, four bits of it
             const uint32_t w = static_cast<const uint32_t*>(A.mask)[row * A.mask_stride + (j >> 6)] >> (4 * ((j >> 3) & 7));
@@ -70,6 +61,11 @@ __device__ __forceinline__ void load_vec(const Args& A, long long row, const T* 
 #pragma unroll
         for (int e = 0; e < N; ++e) out[e] = j + e < end && is_allowed<MASK>(A, row, j + e) ? (float)x[j + e] : -__builtin_huge_valf();
     }
+}
+template <typename T> __device__ __forceinline__ typename Vec<T>::type load_vec(const T* x, int j, int end) {
+    typename Vec<T>::type v = {};
+    if (j + Vec<T>::N <= end) v = *reinterpret_cast<const typename Vec<T>::type*>(x + j);
+    return v;
 }
 
 __device__ __forceinline__ long long action_at(const Args& A, long long i) {
@@ -110,6 +106,7 @@ struct TopList {
     }
     // every lane's candidate (x, j); -inf and NaN are none
     __device__ __forceinline__ void offer(float x, int j, int k) {
+        if (!__any(x >= tau)) return;
         unsigned long long m = __ballot(x > tau || (x == tau && j < tau_i));
         while (m) {
             const int l = first_lane(m);
@@ -144,33 +141,37 @@ __device__ __forceinline__ void carry(Sums& s, float m, float c) {
     s.m = m;
 }
 
+// The alternatives of a part of one tile are taken from the registers.  Over several tiles the list holds vectors instead of elements (the
+// largest of each vector, and the vector's number): a tile is looked at again only if one of its vectors can still enter, and at the end
+// lane r reads the vector of rank r and offers its elements.  The k best elements are in the k best vectors: any other vector's best
+// element has k elements before it, of a larger value or, as vectors are numbered like their elements, of the same value and a lower index.
 template <typename T, int MASK, bool TOP>
 __device__ __forceinline__ void scan(const Args& A, long long row, int begin, int end, Sums& s, TopList& list) {
     constexpr int N = Vec<T>::N, U = PER_LANE / N;
     const T* x = static_cast<const T*>(A.logits) + row * A.row_stride;
     const int lane = lane_id(), k = A.top;
     const float c = A.inv_temperature * LOG2E;
+    const bool one = end - begin <= TILE;
     s.m = LOWEST; s.S = 0.0f; s.D = 0.0f;
+    typename Vec<T>::type raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = load_vec<T>(x, begin + (u * 64 + lane) * N, end);
     for (int j0 = begin; j0 < end; j0 += TILE) {
         float v[PER_LANE], vm[U], tm = -__builtin_huge_valf();
         const int left = (end - j0 + 64 * N - 1) / (64 * N);                      // vectors of this tile that hold anything
-        if (j0 + TILE <= end) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) load_vec<T, MASK, true>(A, row, x, j0 + (u * 64 + lane) * N, end, v + u * N);
-        } else {
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (u < left) load_vec<T, MASK, false>(A, row, x, j0 + (u * 64 + lane) * N, end, v + u * N);
-        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             vm[u] = -__builtin_huge_valf();
             if (u < left) {
+                values<T, MASK>(A, row, x, j0 + (u * 64 + lane) * N, end, raw[u], v + u * N);
 #pragma unroll
                 for (int e = 0; e < N; ++e) vm[u] = fmaxf(vm[u], v[u * N + e]);
             }
             tm = fmaxf(tm, vm[u]);
         }
+        if (j0 + TILE < end)                                                      // the next tile is on its way while this one is summed
+#pragma unroll
+            for (int u = 0; u < U; ++u) raw[u] = load_vec<T>(x, j0 + TILE + (u * 64 + lane) * N, end);
         if (__any(tm > s.m)) carry(s, fmaxf(tm, s.m), c);
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -184,16 +185,29 @@ __device__ __forceinline__ void scan(const Args& A, long long row, int begin, in
             }
         if constexpr (TOP) {
             if (!(list.tau > -__builtin_huge_valf())) list.bound_from_below(tm, k);
-            // elements come in rising vectors: one that equals the last entry of an earlier vector comes behind it
-            if (__any(list.tau_i < j0 ? tm > list.tau : tm >= list.tau)) {
+            if (one) {
 #pragma unroll
                 for (int u = 0; u < U; ++u)
                     if (u < left && __any(vm[u] >= list.tau)) {
 #pragma unroll
                         for (int e = 0; e < N; ++e) list.offer(v[u * N + e], j0 + (u * 64 + lane) * N + e, k);
                     }
+            } else if (__any(tm >= list.tau)) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) list.offer(vm[u], (j0 - begin) / N + u * 64 + lane, k);
             }
         }
+    }
+    if (TOP && !one) {
+        float e[N];
+        const bool have = lane < k && list.i >= 0;
+        const int j = have ? begin + list.i * N : 0, n = have ? end : 0;                         // (a lane without a vector: no element is below 0)
+        values<T, MASK>(A, row, x, j, n, load_vec<T>(x, j, n), e);
+        TopList best;
+        if (list.tau > -__builtin_huge_valf()) { best.tau = list.tau; best.tau_i = 0x7FFFFFFF; }
+#pragma unroll
+        for (int i = 0; i < N; ++i) best.offer(e[i], j + i, k);
+        list = best;
     }
 }
 
@@ -229,9 +243,9 @@ __device__ __forceinline__ void write_row(const Args& A, long long row, const Su
 }
 
 // parts == 1: a wavefront per row.  Otherwise the row is cut into `parts` of `length` elements (whole tiles), a wavefront each, whose sums
-// and lists go to the scratch memory for k_logprobs_join: float4 [rows][parts], values and indexes [rows][parts][top].
+// and lists go to the scratch memory for k_logprobs_join: float4 [rows][parts], values and indexes [rows][top][parts].
 template <typename T, int MASK, bool TOP>
-__global__ __launch_bounds__(256) void k_logprobs(const Args A, int parts, int length) {
+__global__ __launch_bounds__(256, 4) void k_logprobs(const Args A, int parts, int length) {
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     Sums s;
     if (parts == 1) {
@@ -256,8 +270,9 @@ __global__ __launch_bounds__(256) void k_logprobs(const Args A, int parts, int l
         if (TOP && lane_id() < A.top) {
             float* tv = reinterpret_cast<float*>(sums + A.n * parts);
             int* ti = reinterpret_cast<int*>(tv + A.n * parts * A.top);
-            tv[at * A.top + lane_id()] = list.v;
-            ti[at * A.top + lane_id()] = list.i;
+            const long long slot = (row * A.top + lane_id()) * parts + part;
+            tv[slot] = list.v;
+            ti[slot] = list.i;
         }
     }
 }
@@ -281,13 +296,19 @@ __global__ __launch_bounds__(64) void k_logprobs_join(const Args A, int parts) {
         }
         join_lanes(s, c);
         TopList list;
-        if constexpr (TOP) {
-            const int n = parts * A.top;
-            for (int q = 0; q < n; q += 64) {
-                const bool have = q + lane < n;
-                const float x = have ? tv[row * n + q + lane] : -__builtin_huge_valf();
-                if (!(list.tau > -__builtin_huge_valf())) list.bound_from_below(x, A.top);
-                list.offer(x, have ? ti[row * n + q + lane] : -1, A.top);
+        if constexpr (TOP) {                                                      // rank by rank: where no part's next one can enter, none behind it can
+            const long long at = row * parts * A.top;
+            for (int r = 0; r < A.top; ++r) {
+                bool any = false;
+                for (int p0 = 0; p0 < parts; p0 += 64) {
+                    const bool have = p0 + lane < parts;
+                    const float x = have ? tv[at + r * parts + p0 + lane] : -__builtin_huge_valf();
+                    if (!(list.tau > -__builtin_huge_valf())) list.bound_from_below(x, A.top);
+                    if (!__any(x >= list.tau && x > -__builtin_huge_valf())) continue;
+                    any = true;
+                    list.offer(x, have ? ti[at + r * parts + p0 + lane] : -1, A.top);
+                }
+                if (!any) break;
             }
         }
         write_row<T, MASK, TOP>(A, row, s, list);
@@ -308,12 +329,11 @@ __global__ __launch_bounds__(256) void k_logprobs_bwd(const Args A) {
         const T* x = static_cast<const T*>(A.logits) + row * A.row_stride;
         T* out = static_cast<T*>(A.grad) + row * A.grad_stride;
         float v[BWD_PER_LANE], given[BWD_PER_LANE];
+        typename Vec<T>::type raw[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int j = j0 + (u * 64 + lane) * N;
-            if (j0 + BWD_TILE <= V) load_vec<T, MASK, true>(A, row, x, j, V, v + u * N);
-            else load_vec<T, MASK, false>(A, row, x, j, V, v + u * N);
-        }
+        for (int u = 0; u < U; ++u) raw[u] = load_vec<T>(x, j0 + (u * 64 + lane) * N, V);
+#pragma unroll
+        for (int u = 0; u < U; ++u) values<T, MASK>(A, row, x, j0 + (u * 64 + lane) * N, V, raw[u], v + u * N);
         const float4 st = *reinterpret_cast<const float4*>(A.stats + 4 * row);
         const float m = st.x, rS = 1.0f / st.y, lnS = logf(st.y), H = st.z, h = A.g_entropy ? A.g_entropy[row] : 0.0f;
         // lane k has the k-th given action; those of this tile go to the lanes that hold their elements, in the order of k

@@ -5,6 +5,8 @@ float32.  This optimiser takes any module's parameters, in float32, bfloat16 or 
 """
 import ctypes as C
 import math
+from array import array
+from operator import attrgetter
 
 import torch
 
@@ -13,6 +15,9 @@ from . import _lib
 BLOCK = 128                         # elements that share a scale in 8-bit moments; every tensor's part of the states is padded to it
 TENSORS, BLOCKS = 96, 2048          # of one launch (ckr_adamw.hip)
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+# accessors for map(): a step looks at every parameter and gradient
+_SHAPE, _DTYPE, _GRAD = attrgetter("shape"), attrgetter("dtype"), attrgetter("grad")
+_STRIDE, _DEVICE, _POINTER = torch.Tensor.stride, torch.Tensor.get_device, torch.Tensor.data_ptr
 
 
 class AdamWArgs(C.Structure):
@@ -38,13 +43,10 @@ class _Batch:
     """The tensors of one group and type: what one call of ckr_adamw_step takes."""
 
     def __init__(self, group, dtype, params, offsets, first):
-        n = len(params)
-        self.group, self.dtype, self.params, self.first, self.n = group, dtype, params, first, n
-        self.layouts = [_layout(p) for p in params]
-        self.strides = [p.stride() for p in params]
-        self.shapes = [p.shape for p in params]
-        self.sizes = (C.c_int64 * n)(*[p.numel() for p in params])
-        self.offsets = (C.c_int64 * n)(*offsets)
+        self.group, self.dtype, self.params, self.first, self.n = group, dtype, params, first, len(params)
+        self.sizes = (C.c_int64 * self.n)(*[p.numel() for p in params])
+        self.offsets = (C.c_int64 * self.n)(*offsets)
+        self.seen = None                                               # the group's hyperparameters that passed the checks last
 
 
 class AdamW:
@@ -124,11 +126,19 @@ class AdamW:
         # partial sums of the norm: one launch for each run of up to TENSORS tensors of one type
         launches = sum((b.n + TENSORS - 1) // TENSORS for b in self._batches)
         self._parts, self._norm = (z(max(1, launches) * BLOCKS, torch.float64), z(2, torch.float64)) if self.max_norm is not None else (None, None)
-        self._sizes_all = (C.c_int64 * first)(*[n for b in self._batches for n in b.sizes])
-        self._dtypes_all = (C.c_int32 * first)(*[DTYPES[b.dtype] for b in self._batches for _ in range(b.n)])
+        self._every = [p for b in self._batches for p in b.params]     # in the order of the batches
+        self._sizes_all = (C.c_int64 * first)(*[p.numel() for p in self._every])
+        self._dtypes_all = (C.c_int32 * first)(*[DTYPES[p.dtype] for p in self._every])
+        self._layouts = [_layout(p) for p in self._every]
+        self._shape_of, self._stride_of, self._type_of = ([f(p) for p in self._every] for f in (_SHAPE, _STRIDE, _DTYPE))
+        self._device_of = [dev.index] * first
         self._streams = {torch.cuda.current_stream(dev).cuda_stream}
         torch.cuda.current_stream(dev).synchronize()                   # a step on any stream finds the states in place
         self._L = _lib.load()
+        ptr = lambda t: None if t is None else t.data_ptr()
+        scales = (None, None) if self.scales is None else (self.scales[0].data_ptr(), self.scales[1].data_ptr())
+        self._states = (ptr(self.master), self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr()) + scales
+        self._steps_ptr, self._ticket_ptr, self._norm_ptr = self.steps.data_ptr(), self._ticket.data_ptr(), ptr(self._norm)
 
     def _check_group(self, g):
         lr = g["lr"]
@@ -150,30 +160,31 @@ class AdamW:
         """p's part of a flat buffer, in p's own shape and order of dimensions."""
         return flat.as_strided(p.shape, p.stride(), flat.storage_offset() + offset) if p.numel() else flat.new_empty(p.shape)
 
-    def _gradients(self, b, keep):
-        """Device pointers of a batch's parameters and gradients (0: none); a gradient that lies otherwise than its parameter is copied."""
-        ps, gs = [], []
-        for p, strides, shape, layout in zip(b.params, b.strides, b.shapes, b.layouts):
-            g = p.grad
-            if g is None:
-                ps.append(0)
-                gs.append(0)
-                continue
-            if p.stride() != strides or p.shape != shape or p.dtype != b.dtype or p.device != self.device:
-                raise ValueError("a parameter's shape, strides, type or device changed after the optimiser was made")
-            if g.stride() != strides:
-                if g.layout != torch.strided:
-                    raise ValueError("sparse gradients are not supported")
-                if g.shape != shape:
-                    raise ValueError("a gradient of shape %s for a parameter of shape %s" % (list(g.shape), list(shape)))
-                if _layout(g) != layout:
-                    g = torch.empty_strided(shape, strides, dtype=b.dtype, device=self.device).copy_(g)
-                    keep.append(g)
-            if g.dtype != b.dtype or g.device != self.device:
-                raise ValueError("a gradient must have its parameter's type and device")
-            ps.append(p.data_ptr())
-            gs.append(g.data_ptr())
-        return (C.c_void_p * b.n)(*ps), (C.c_void_p * b.n)(*gs)
+    def _pointers(self):
+        """Device addresses of all parameters and gradients in the order of the batches (0: no gradient), and copies of gradients that lie
+        otherwise than their parameters."""
+        ps = self._every
+        if list(map(_SHAPE, ps)) != self._shape_of or list(map(_STRIDE, ps)) != self._stride_of or list(map(_DTYPE, ps)) != self._type_of \
+                or list(map(_DEVICE, ps)) != self._device_of:
+            raise ValueError("a parameter's shape, strides, type or device changed after the optimiser was made")
+        gs, keep = list(map(_GRAD, ps)), []
+        if any(g is None for g in gs) or list(map(_STRIDE, gs)) != self._stride_of or list(map(_SHAPE, gs)) != self._shape_of \
+                or list(map(_DTYPE, gs)) != self._type_of or list(map(_DEVICE, gs)) != self._device_of:
+            gs = [self._gradient(i, g, keep) for i, g in enumerate(gs)]
+            return array("Q", map(_POINTER, ps)), array("Q", (0 if g is None else g.data_ptr() for g in gs)), keep
+        return array("Q", map(_POINTER, ps)), array("Q", map(_POINTER, gs)), keep
+
+    def _gradient(self, i, g, keep):
+        if g is None:
+            return None
+        if g.layout != torch.strided:
+            raise ValueError("sparse gradients are not supported")
+        if g.shape != self._shape_of[i] or g.dtype != self._type_of[i] or g.device != self.device:
+            raise ValueError("a gradient must have its parameter's shape, type and device")
+        if _layout(g) != self._layouts[i]:
+            g = torch.empty_strided(g.shape, self._stride_of[i], dtype=g.dtype, device=g.device).copy_(g)
+            keep.append(g)
+        return g
 
     @torch.no_grad()
     def step(self):
@@ -184,37 +195,33 @@ class AdamW:
         return self._step()
 
     def _step(self):
-        L = self._L
-        cur = torch.cuda.current_stream(self.device)
-        s = cur.cuda_stream
+        L, s = self._L, _lib.raw_stream(self.device.index)
         if s not in self._streams:                                     # the allocator has to know before it hands the memory on
             self._streams.add(s)
             for t in (self.exp_avg, self.exp_avg_sq, self.scales, self.master, self.steps, self._ticket, self._parts, self._norm):
                 if t is not None:
-                    t.record_stream(cur)
-        keep, ptrs = [], []
+                    t.record_stream(torch.cuda.current_stream(self.device))
         for b in self._batches:
-            self._check_group(b.group)
-            ptrs.append(self._gradients(b, keep))
-        if self.max_norm is not None:
-            grads = (C.c_void_p * len(self._sizes_all))(*[g for _, gs in ptrs for g in gs])
-            _lib.check(L.ckr_grad_norm(len(grads), self._sizes_all, grads, self._dtypes_all, self.max_norm, self._parts.data_ptr(),
-                                       self._parts.numel(), self._ticket.data_ptr() + 4, self._norm.data_ptr(), s))
-        scales = (None, None) if self.scales is None else (self.scales[0].data_ptr(), self.scales[1].data_ptr())
-        done = []
-        for b, (ps, gs) in zip(self._batches, ptrs):
             g = b.group
-            lr, (b1, b2) = g["lr"], g["betas"]
+            now = g["lr"], g["betas"], g["eps"], g["weight_decay"]
+            if b.seen is None or not all(x is y for x, y in zip(now, b.seen)):
+                self._check_group(g)
+                b.seen = now
+        ps, gs, keep = self._pointers()
+        p0, g0 = ps.buffer_info()[0], gs.buffer_info()[0]
+        if self.max_norm is not None:
+            _lib.check(L.ckr_grad_norm(len(gs), self._sizes_all, g0, self._dtypes_all, self.max_norm, self._parts.data_ptr(), self._parts.numel(),
+                                       self._ticket.data_ptr() + 4, self._norm.data_ptr(), s))
+        for b in self._batches:
+            lr, (b1, b2), eps, decay = b.seen
             on_device = isinstance(lr, torch.Tensor)
-            a = AdamWArgs(C.addressof(b.sizes), C.addressof(b.offsets), C.addressof(ps), C.addressof(gs),
-                          None if self.master is None else self.master.data_ptr(), self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), *scales,
-                          self.steps.data_ptr() + 4 * b.first, self._ticket.data_ptr(), lr.data_ptr() if on_device else None,
-                          None if self._norm is None else self._norm.data_ptr(), 0.0 if on_device else float(lr), float(b1), float(b2),
-                          float(g["weight_decay"]), self.seed, float(g["eps"]), b.n, DTYPES[b.dtype], self.state_bits)
+            a = AdamWArgs(C.addressof(b.sizes), C.addressof(b.offsets), p0 + 8 * b.first, g0 + 8 * b.first, *self._states, self._steps_ptr + 4 * b.first, self._ticket_ptr,
+                          lr.data_ptr() if on_device else None, self._norm_ptr, 0.0 if on_device else float(lr), float(b1), float(b2), float(decay), self.seed,
+                          float(eps), b.n, DTYPES[b.dtype], self.state_bits)
             _lib.check(L.ckr_adamw_step(C.byref(a), s))
-            done += [p for p, ptr in zip(b.params, gs) if ptr]
-        if done:
-            torch.autograd.graph.increment_version(done)               # a backward pass over what it saved before the step is refused
+        stepped = self._every if 0 not in gs else [p for p, g in zip(self._every, gs) if g]
+        if stepped:
+            torch.autograd.graph.increment_version(stepped)            # a backward pass over what it saved before the step is refused
 
     @property
     def grad_norm(self):
@@ -238,10 +245,15 @@ class AdamW:
             return self.exp_avg, self.exp_avg_sq
         m, v = (torch.empty((self.total,), dtype=torch.float32, device=self.device) for _ in range(2))
         if self.total:
-            with torch.cuda.device(self.device):
-                _lib.check(self._L.ckr_adamw_read_moments(self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), self.scales[0].data_ptr(), self.scales[1].data_ptr(),
-                                                          self.total, m.data_ptr(), v.data_ptr(), torch.cuda.current_stream(self.device).cuda_stream))
+            self._on_device(self._L.ckr_adamw_read_moments, *self._states[1:], self.total, m.data_ptr(), v.data_ptr())
         return m, v
+
+    def _on_device(self, fn, *args):
+        if torch.cuda.current_device() == self.device.index:
+            _lib.check(fn(*args, _lib.raw_stream(self.device.index)))
+        else:
+            with torch.cuda.device(self.device):
+                _lib.check(fn(*args, _lib.raw_stream(self.device.index)))
 
     def split(self, flat):
         """Views of a flat tensor of moments (or of `master`), one for each parameter, in its shape."""
@@ -269,9 +281,7 @@ class AdamW:
             self.exp_avg.copy_(flat[0])
             self.exp_avg_sq.copy_(flat[1])
         elif self.total:
-            with torch.cuda.device(self.device):
-                _lib.check(self._L.ckr_adamw_write_moments(flat[0].data_ptr(), flat[1].data_ptr(), self.total, self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(),
-                                                           self.scales[0].data_ptr(), self.scales[1].data_ptr(), torch.cuda.current_stream(self.device).cuda_stream))
+            self._on_device(self._L.ckr_adamw_write_moments, flat[0].data_ptr(), flat[1].data_ptr(), self.total, *self._states[1:])
         self.steps.fill_(int(step))
 
     def state_dict(self):

@@ -5,6 +5,7 @@ The reference reads its policy as one dense masked softmax (Checkers.predict, Ch
 counterpart of these.  All tensors live on a `cuda` (HIP) device; there is no CPU fallback.
 """
 import ctypes as C
+import functools
 from collections import namedtuple
 
 import torch
@@ -32,43 +33,41 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _args(x, actions, mask, mask_kind, top, inv_temperature):
-    n, v = x.shape
-    a = LogprobsArgs()
-    a.logits, a.n, a.v, a.row_stride, a.dtype = x.data_ptr(), n, v, x.stride(0) if n > 1 else v, DTYPES[x.dtype]
-    if actions is not None:
-        a.actions, a.action_bytes, a.n_given = actions.data_ptr(), actions.element_size(), actions.shape[1]
-    if mask is not None:
-        a.mask, a.mask_kind, a.mask_stride = mask.data_ptr(), mask_kind, mask.stride(0) if mask.shape[0] > 1 else 0
-    a.top, a.inv_temperature = top, inv_temperature
-    return a
+@functools.lru_cache(maxsize=1024)
+def _scratch_bytes(n, v, top):
+    """ckr_logprobs_scratch: a function of the sizes alone."""
+    bytes_ = _lib.load().ckr_logprobs_scratch(C.byref(LogprobsArgs(n=n, v=v, top=top, inv_temperature=1.0, logits=16)))
+    if bytes_ < 0:
+        _lib.check(int(bytes_))
+    return bytes_
 
 
 def _call(fn, args, device):
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        _lib.check(fn(C.byref(args), stream))
+    """Launch on the current stream of `device`."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        _lib.check(fn(C.byref(args), _lib.raw_stream(index)))
     else:
         with torch.cuda.device(device):
-            _lib.check(fn(C.byref(args), stream))
+            _lib.check(fn(C.byref(args), _lib.raw_stream(index)))
 
 
 def _forward(x, actions, mask, mask_kind, top, inv_temperature, want_stats):
     """x [n, v] (last dimension dense), actions [n, k] or None, mask [n or 1, ...] or None."""
-    L, n, dev = _lib.load(), x.shape[0], x.device
-    logp = None if actions is None else torch.empty(actions.shape, dtype=torch.float32, device=dev)
-    entropy = torch.empty((n,), dtype=torch.float32, device=dev)
-    top_action = torch.empty((n, top), dtype=torch.int64, device=dev) if top else None
-    top_logp = torch.empty((n, top), dtype=torch.float32, device=dev) if top else None
-    stats = torch.empty((n, 4), dtype=torch.float32, device=dev) if want_stats else None
-    a = _args(x, actions, mask, mask_kind, top, inv_temperature)
-    a.logp, a.entropy, a.top_action, a.top_logp, a.stats = _ptr(logp), entropy.data_ptr(), _ptr(top_action), _ptr(top_logp), _ptr(stats)
-    a.scratch_bytes = L.ckr_logprobs_scratch(C.byref(a))
-    if a.scratch_bytes < 0:
-        _lib.check(int(a.scratch_bytes))
-    scratch = torch.empty((a.scratch_bytes,), dtype=torch.uint8, device=dev) if a.scratch_bytes else None
-    a.scratch = _ptr(scratch)
-    _call(L.ckr_logprobs_forward, a, dev)
+    (n, v), dev, f32 = x.shape, x.device, torch.float32
+    empty = torch.empty
+    logp = None if actions is None else empty(actions.shape, dtype=f32, device=dev)
+    entropy = empty(n, dtype=f32, device=dev)
+    top_action = top_logp = None
+    if top:
+        top_action, top_logp = empty((n, top), dtype=torch.int64, device=dev), empty((n, top), dtype=f32, device=dev)
+    stats = empty((n, 4), dtype=f32, device=dev) if want_stats else None
+    need = _scratch_bytes(n, v, top)
+    scratch = empty(need, dtype=torch.uint8, device=dev) if need else None
+    a = LogprobsArgs(x.data_ptr(), _ptr(actions), _ptr(mask), _ptr(logp), entropy.data_ptr(), _ptr(top_action), _ptr(top_logp), _ptr(stats),
+                     None, None, None, _ptr(scratch), n, v, x.stride(0) if n > 1 else v, mask.stride(0) if mask is not None and mask.shape[0] > 1 else 0, 0, need,
+                     DTYPES[x.dtype], mask_kind, 0 if actions is None else actions.element_size(), 0 if actions is None else actions.shape[1], top, inv_temperature)
+    _call(_lib.load().ckr_logprobs_forward, a, dev)
     return logp, entropy, top_action, top_logp, stats
 
 
@@ -92,8 +91,11 @@ class _Logprobs(torch.autograd.Function):
             actions = None
         grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         g_logp, g_entropy = (None if g is None else g.float().contiguous() for g in (g_logp, g_entropy))
-        a = _args(x, actions, mask, ctx.mask_kind, 0, ctx.inv_temperature)
-        a.stats, a.g_logp, a.g_entropy, a.grad, a.grad_stride = stats.data_ptr(), _ptr(g_logp), _ptr(g_entropy), grad.data_ptr(), x.shape[1]
+        n, v = x.shape
+        a = LogprobsArgs(x.data_ptr(), _ptr(actions), _ptr(mask), None, None, None, None, stats.data_ptr(), _ptr(g_logp), _ptr(g_entropy), grad.data_ptr(), None,
+                         n, v, x.stride(0) if n > 1 else v, mask.stride(0) if mask is not None and mask.shape[0] > 1 else 0, v, 0,
+                         DTYPES[x.dtype], ctx.mask_kind, 0 if actions is None else actions.element_size(), 0 if actions is None else actions.shape[1], 0,
+                         ctx.inv_temperature)
         _call(_lib.load().ckr_logprobs_backward, a, x.device)
         return (grad,) + (None,) * 5
 
@@ -160,7 +162,9 @@ def action_logprobs(logits, actions=None, mask=None, top=0, temperature=1.0):
         shape = actions.shape
         if shape != lead and (len(shape) != len(lead) + 1 or shape[:-1] != lead or not 1 <= shape[-1] <= MOST):
             raise ValueError("actions must have the shape %s or %s + [1 .. %d], got %s" % (list(lead), list(lead), MOST, list(shape)))
-        actions = actions.reshape(x.shape[0], 1 if shape == lead else shape[-1]).contiguous()
+        if len(shape) != 2 or shape == lead:
+            actions = actions.reshape(x.shape[0], 1 if shape == lead else shape[-1])
+        actions = actions.contiguous()
     mask_kind = MASK_NONE
     if mask is not None:
         mask, mask_kind = _check_mask(mask, lead, v, logits.device)

@@ -455,6 +455,22 @@ def test_moments_in_and_out(bits):
         opt.load_moments(again[0][:5], again[1], 1)
 
 
+def test_moments_of_steps_come_back_as_they_are():
+    """Blocks whose largest value was rounded up to the next power of two, and what lies 14 powers below it, too."""
+    from checkers_mcts_amd import optim
+    n = 128 * 600
+    for seed in range(3):
+        p = torch.zeros(n, device="cuda", requires_grad=True)
+        opt = optim.AdamW([p], state_bits=8, seed=seed)
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        p.grad = (1.9 + 0.1 * torch.rand((n,), generator=g, device="cuda")) * 2.0 ** -torch.randint(0, 18, (n,), generator=g, device="cuda").float()
+        opt.step()
+        before = [t.clone() for t in opt.moments()]
+        other = optim.AdamW([p], state_bits=8)
+        other.load_moments(*before, 1)
+        assert all(torch.equal(a, b) for a, b in zip(other.moments(), before))
+
+
 def test_refusals():
     from checkers_mcts_amd import optim
     p = torch.zeros(100, device="cuda", requires_grad=True)
