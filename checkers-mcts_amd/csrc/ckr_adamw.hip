@@ -45,14 +45,36 @@ struct Hyper {
     float eps;
 };
 
-// the tensor that chunk c belongs to
+// The tensor that chunk c belongs to, from one load of the whole table: kernel arguments lie in host memory, and each step of a bisection
+// would wait for them anew.
 __device__ __forceinline__ int tensor_of(const TensorTable& T, unsigned c) {
-    int lo = 0, hi = T.tensors;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (T.first[mid] <= c) lo = mid; else hi = mid;
+    static_assert(TENSORS <= 128, "two entries a lane");
+    const int lane = lane_id();
+    const unsigned a = T.first[min(lane, T.tensors)], b = T.first[min(lane + 64, T.tensors)];
+    const int n = __popcll(__ballot(lane < T.tensors && a <= c)) + __popcll(__ballot(lane + 64 < T.tensors && b <= c));
+    return __builtin_amdgcn_readfirstlane(n - 1);
+}
+
+// True in the workgroup that arrives last of `total` (numbered `number`).  All threads call it; what a workgroup did before is done, and what
+// other workgroups are to read of it has been stored with device-scope atomics (no cache is written back for it).  One counter for
+// all of them would be their queue: 690 arrivals took 8 us.  32 counters, a cache line each, and one for their last ones.  All are 0 again afterwards.
+__device__ __forceinline__ bool arrives_last(unsigned* tickets, unsigned number, unsigned total) {
+    __shared__ unsigned last;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (!threadIdx.x) {
+        const unsigned line = number & 31u, of_line = (total - line + 31u) / 32u, lines = total < 32u ? total : 32u;
+        last = 0u;
+        if (__hip_atomic_fetch_add(tickets + 32 * (1 + line), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == of_line - 1u) {
+            __hip_atomic_store(tickets + 32 * (1 + line), 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (__hip_atomic_fetch_add(tickets, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == lines - 1u) {
+                __hip_atomic_store(tickets, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                last = 1u;
+            }
+        }
     }
-    return lo;
+    __syncthreads();
+    return last != 0u;
 }
 
 // ---- the 8-bit formats, on the high word of a double: 11 exponent bits, the first 20 bits of the mantissa ---------------------------
@@ -93,87 +115,115 @@ __device__ __forceinline__ unsigned row16_max(unsigned v) {                     
     return v;
 }
 
+// ---- 8 consecutive elements of a thread, in 16-byte accesses that start at any element -------------------------------------------------
+template <typename T> struct Eight { typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T)))); };
+template <typename T> __device__ __forceinline__ void load8(const T* p, long long left, float* out) {       // left <= 0: none of them, zeros
+    if (left >= 8) {
+        const typename Eight<T>::type v = *reinterpret_cast<const typename Eight<T>::type*>(p);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) out[j] = (float)v[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) out[j] = j < left ? (float)p[j] : 0.0f;
+    }
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, long long left, const float* x) {
+    if (left >= 8) {
+        typename Eight<T>::type v;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (T)x[j];
+        *reinterpret_cast<typename Eight<T>::type*>(p) = v;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < left) p[j] = (T)x[j];
+    }
+}
+
+// chunks [c, end) of this workgroup: an even share, in one piece, so that a tensor is looked up once
+__device__ __forceinline__ unsigned share(unsigned chunks, unsigned b) { return (unsigned)((unsigned long long)chunks * b / gridDim.x); }
+
 // ---- the update: a thread has 8 consecutive elements, 16 lanes a block of 128 --------------------------------------------------------
 template <typename T, int BITS>
 __global__ __launch_bounds__(256) void k_adamw(const TensorTable tab, const Hyper H) {
-    __shared__ unsigned last;
     const double lr = H.d_lr ? (double)*H.d_lr : H.lr;
     const double c = H.norm ? H.norm[1] : 1.0;
     const float decay = (float)(1.0 - lr * H.weight_decay);
-    for (unsigned ch = blockIdx.x; ch < tab.first[tab.tensors]; ch += gridDim.x) {
-        const int i = tensor_of(tab, ch);
-        if (!tab.g[i]) continue;
+    const unsigned chunks = tab.first[tab.tensors], end = share(chunks, blockIdx.x + 1);
+    unsigned ch = share(chunks, blockIdx.x);
+    for (int i = tensor_of(tab, ch); ch < end; ++i) {                             // (tensors without a gradient have no chunks)
+        const unsigned stop = min(end, tab.first[i + 1]);
+        if (ch >= stop) continue;
         const int t = H.step[i] + 1;
         const double bc1 = -expm1(t * H.ln_beta1), bc2 = -expm1(t * H.ln_beta2);
         const float rate = (float)(lr / bc1), rs = (float)(1.0 / sqrt(bc2));
-        const long long e0 = (long long)(ch - tab.first[i]) * CHUNK + threadIdx.x * 8, left = tab.n[i] - e0;
-        const long long s0 = tab.off[i] + e0;                                     // of the states: whole blocks, so never past the end
-        T* p = static_cast<T*>(tab.p[i]) + e0;
-        const T* g = static_cast<const T*>(tab.g[i]) + e0;
-        const long long blocks_end = (tab.n[i] + 127) / 128 * 128;
-        const bool in = e0 < blocks_end;
-        float w[8], gr[8], mf[8], vf[8];
+        T* const p = static_cast<T*>(tab.p[i]);
+        const T* const g = static_cast<const T*>(tab.g[i]);
+        const long long n = tab.n[i], off = tab.off[i];
+        for (; ch < stop; ++ch) {
+            const long long e0 = (long long)(ch - tab.first[i]) * CHUNK + threadIdx.x * 8, left = n - e0;
+            const long long s0 = off + e0;                                        // of the states: whole blocks of 128
+            const bool in = e0 < (n + 127) / 128 * 128;
+            float w[8], gr[8], mf[8], vf[8];
+            load8(g + e0, left, gr);
+            if constexpr (sizeof(T) == 4) load8(p + e0, left, w);
+            else load8(H.master + s0, in ? 8 : 0, w);
+            if constexpr (BITS == 32) {
+                float* const m = static_cast<float*>(H.m) + s0;
+                float* const v = static_cast<float*>(H.v) + s0;
+                const float b1 = (float)H.beta1, b2 = (float)H.beta2, a1 = (float)(1.0 - H.beta1), a2 = (float)(1.0 - H.beta2), cf = (float)c;
+                load8(m, in ? 8 : 0, mf);
+                load8(v, in ? 8 : 0, vf);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const bool have = j < left;
-            gr[j] = have ? (float)g[j] : 0.0f;
-            w[j] = !have ? 0.0f : sizeof(T) == 4 ? (float)p[j] : H.master[s0 + j];
-        }
-        if constexpr (BITS == 32) {
-            float* m = static_cast<float*>(H.m) + s0;
-            float* v = static_cast<float*>(H.v) + s0;
-            const float b1 = (float)H.beta1, b2 = (float)H.beta2, a1 = (float)(1.0 - H.beta1), a2 = (float)(1.0 - H.beta2), cf = (float)c;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (in) {
+                for (int j = 0; j < 8; ++j) {
                     const float x = gr[j] * cf;
-                    m[j] = mf[j] = b1 * m[j] + a1 * x;
-                    v[j] = vf[j] = b2 * v[j] + a2 * x * x;
+                    mf[j] = b1 * mf[j] + a1 * x;
+                    vf[j] = b2 * vf[j] + a2 * x * x;
                 }
-        } else {
-            uint8_t* m = static_cast<uint8_t*>(H.m) + s0;
-            uint8_t* v = static_cast<uint8_t*>(H.v) + s0;
-            const int ms = in ? H.m_scale[s0 / 128] : 1, vs = in ? H.v_scale[s0 / 128] : 1;
-            double md[8], vd[8];
-            unsigned hm = 0, hv = 0;
+                store8(m, in ? 8 : 0, mf);
+                store8(v, in ? 8 : 0, vf);
+            } else {
+                uint2* const m = reinterpret_cast<uint2*>(static_cast<uint8_t*>(H.m) + s0);
+                uint2* const v = reinterpret_cast<uint2*>(static_cast<uint8_t*>(H.v) + s0);
+                const uint2 mc = in ? *m : make_uint2(0, 0), vc = in ? *v : make_uint2(0, 0);
+                const int ms = in ? H.m_scale[s0 / 128] : 1, vs = in ? H.v_scale[s0 / 128] : 1;
+                double md[8], vd[8];
+                unsigned hm = 0, hv = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const double x = (double)gr[j] * c;
-                md[j] = H.beta1 * decode_m(in ? m[j] : 0u, ms) + (1.0 - H.beta1) * x;
-                vd[j] = H.beta2 * decode_v(in ? v[j] : 0u, vs) + (1.0 - H.beta2) * x * x;
-                hm = max(hm, high_word(md[j])); hv = max(hv, high_word(vd[j]));
-                mf[j] = (float)md[j]; vf[j] = (float)vd[j];
-            }
-            const int ms1 = scale_byte(row16_max(hm)), vs1 = scale_byte(row16_max(hv));
-            const unsigned long long grp = (unsigned long long)s0 / 8;
-            const u32x4 r = philox((unsigned)H.seed, (unsigned)(H.seed >> 32), (unsigned)grp, (unsigned)(grp >> 32), (unsigned)t, 0u);
-            const unsigned rw[4] = {r.x, r.y, r.z, r.w};
-            if (in) {
+                for (int j = 0; j < 8; ++j) {
+                    const double x = (double)gr[j] * c;
+                    md[j] = H.beta1 * decode_m(((j < 4 ? mc.x : mc.y) >> (8 * (j & 3))) & 255u, ms) + (1.0 - H.beta1) * x;
+                    vd[j] = H.beta2 * decode_v(((j < 4 ? vc.x : vc.y) >> (8 * (j & 3))) & 255u, vs) + (1.0 - H.beta2) * x * x;
+                    hm = max(hm, high_word(md[j])); hv = max(hv, high_word(vd[j]));
+                    mf[j] = (float)md[j]; vf[j] = (float)vd[j];
+                }
+                const int ms1 = scale_byte(row16_max(hm)), vs1 = scale_byte(row16_max(hv));
+                const unsigned long long grp = (unsigned long long)s0 / 8;
+                const u32x4 r = philox((unsigned)H.seed, (unsigned)(H.seed >> 32), (unsigned)grp, (unsigned)(grp >> 32), (unsigned)t, 0u);
+                const unsigned rw[4] = {r.x, r.y, r.z, r.w};
+                unsigned mo[2] = {0, 0}, vo[2] = {0, 0};
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {                                     // 16 of 32 random bits for v, the others for m: 2 r + 1 of 2^17
                     const unsigned lo = rw[j >> 1] & 0xFFFFu, hi = rw[j >> 1] >> 16;
-                    m[j] = (uint8_t)encode_m(md[j], ms1, 2u * (j & 1 ? lo : hi) + 1u);
-                    v[j] = (uint8_t)encode_v(vd[j], vs1, 2u * (j & 1 ? hi : lo) + 1u);
+                    mo[j >> 2] |= encode_m(md[j], ms1, 2u * (j & 1 ? lo : hi) + 1u) << (8 * (j & 3));
+                    vo[j >> 2] |= encode_v(vd[j], vs1, 2u * (j & 1 ? hi : lo) + 1u) << (8 * (j & 3));
                 }
-                if ((threadIdx.x & 15) == 0) { H.m_scale[s0 / 128] = (uint8_t)ms1; H.v_scale[s0 / 128] = (uint8_t)vs1; }
+                if (in) {
+                    *m = make_uint2(mo[0], mo[1]);
+                    *v = make_uint2(vo[0], vo[1]);
+                    if ((threadIdx.x & 15) == 0) { H.m_scale[s0 / 128] = (uint8_t)ms1; H.v_scale[s0 / 128] = (uint8_t)vs1; }
+                }
             }
-        }
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < left) {
-                const float x = w[j] * decay - rate * (mf[j] / (sqrtf(vf[j]) * rs + H.eps));
-                if constexpr (sizeof(T) == 4) p[j] = x;
-                else { H.master[s0 + j] = x; p[j] = (T)x; }
-            }
+            for (int j = 0; j < 8; ++j) w[j] = w[j] * decay - rate * (mf[j] / (sqrtf(vf[j]) * rs + H.eps));
+            if constexpr (sizeof(T) != 4) store8(H.master + s0, left < 8 ? left : 8, w);
+            store8(p + e0, left, w);
+        }
     }
     // The workgroup that ends last advances the step counters: by then every other one has read them.
-    __syncthreads();
-    if (!threadIdx.x) last = __hip_atomic_fetch_add(H.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
-    __syncthreads();
-    if (!last) return;
+    if (!arrives_last(H.ticket, blockIdx.x, gridDim.x)) return;
     for (int i = threadIdx.x; i < tab.tensors; i += 256)
         if (tab.g[i]) H.step[i] += 1;
-    if (!threadIdx.x) __hip_atomic_store(H.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // ---- the global norm: every workgroup's sum of squares in parts[base + blockIdx], the last of all `total` workgroups adds them in order --
@@ -181,28 +231,34 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_grad_norm(const TensorTable tab, double max_norm, double* __restrict__ parts, int base, int total,
                                                    unsigned* __restrict__ ticket, double* __restrict__ out) {
     __shared__ double red[256];
-    __shared__ unsigned last;
     double s = 0.0;
-    for (unsigned ch = blockIdx.x; ch < tab.first[tab.tensors]; ch += gridDim.x) {
-        const int i = tensor_of(tab, ch);
-        if (!tab.g[i]) continue;
-        const long long e0 = (long long)(ch - tab.first[i]) * CHUNK + threadIdx.x * 8, left = tab.n[i] - e0;
-        const T* g = static_cast<const T*>(tab.g[i]) + e0;
+    const unsigned chunks = tab.first[tab.tensors], end = share(chunks, blockIdx.x + 1);
+    unsigned ch = share(chunks, blockIdx.x);
+    for (int i = tensor_of(tab, ch); ch < end; ++i) {
+        const unsigned stop = min(end, tab.first[i + 1]);
+        if (ch >= stop) continue;
+        const T* const g = static_cast<const T*>(tab.g[i]) + threadIdx.x * 8;
+        const long long n = tab.n[i] - threadIdx.x * 8;
+        while (ch < stop) {                                                       // four chunks' loads at a time
+            float x[4][8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < left) { const double x = (double)(float)g[j]; s += x * x; }
+            for (int q = 0; q < 4; ++q) {
+                const long long e0 = (long long)(ch + q - tab.first[i]) * CHUNK;
+                load8(g + e0, ch + q < stop ? n - e0 : 0, x[q]);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s = __builtin_fma((double)x[q][j], (double)x[q][j], s);
+            ch += 4;
+        }
+        ch = stop;
     }
     red[threadIdx.x] = s;
     __syncthreads();
     for (int d = 128; d >= 1; d >>= 1) { if ((int)threadIdx.x < d) red[threadIdx.x] += red[threadIdx.x + d]; __syncthreads(); }
-    // the part travels as a device-scope atomic and has been acknowledged before the ticket is taken: no cache is written back for it
-    if (!threadIdx.x) {
-        __hip_atomic_store(parts + base + blockIdx.x, red[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __builtin_amdgcn_s_waitcnt(0);
-        last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)total - 1u;
-    }
-    __syncthreads();
-    if (!last) return;
+    if (!threadIdx.x) __hip_atomic_store(parts + base + blockIdx.x, red[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (!arrives_last(ticket, (unsigned)base + blockIdx.x, (unsigned)total)) return;
     s = 0.0;
     for (int b = threadIdx.x; b < total; b += 256) s += __hip_atomic_load(parts + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     red[threadIdx.x] = s;
@@ -212,18 +268,23 @@ __global__ __launch_bounds__(256) void k_grad_norm(const TensorTable tab, double
     const double norm = sqrt(red[0]), c = max_norm / (norm + 1e-6);
     out[0] = norm;
     out[1] = c >= 1.0 ? 1.0 : c;                                                  // NaN stays NaN
-    __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // ---- reading and writing 8-bit moments (n a multiple of 128) -------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void k_moments_read(const uint8_t* __restrict__ m, const uint8_t* __restrict__ v, const uint8_t* __restrict__ m_scale,
                                                       const uint8_t* __restrict__ v_scale, long long n, float* __restrict__ m_out, float* __restrict__ v_out) {
-    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (long long)gridDim.x * 2048)
+    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (long long)gridDim.x * 2048) {
+        const uint2 mc = *reinterpret_cast<const uint2*>(m + i), vc = *reinterpret_cast<const uint2*>(v + i);
+        const int ms = m_scale[i / 128], vs = v_scale[i / 128];
+        float mo[8], vo[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            m_out[i + j] = (float)decode_m(m[i + j], m_scale[i / 128]);
-            v_out[i + j] = (float)decode_v(v[i + j], v_scale[i / 128]);
+            mo[j] = (float)decode_m(((j < 4 ? mc.x : mc.y) >> (8 * (j & 3))) & 255u, ms);
+            vo[j] = (float)decode_v(((j < 4 ? vc.x : vc.y) >> (8 * (j & 3))) & 255u, vs);
         }
+        store8(m_out + i, 8, mo);
+        store8(v_out + i, 8, vo);
+    }
 }
 __global__ __launch_bounds__(256) void k_moments_write(const float* __restrict__ m_in, const float* __restrict__ v_in, long long n, uint8_t* __restrict__ m,
                                                        uint8_t* __restrict__ v, uint8_t* __restrict__ m_scale, uint8_t* __restrict__ v_scale) {
@@ -256,7 +317,7 @@ static void fill_table(TensorTable& T, int count, int k, const int64_t* sizes, c
     }
     T.first[T.tensors] = chunks;
 }
-static unsigned grid_of(const TensorTable& T) { const unsigned c = T.first[T.tensors]; return c < 1u ? 1u : c < (unsigned)BLOCKS ? c : (unsigned)BLOCKS; }
+static unsigned grid_of(const TensorTable& T, unsigned each = 1) { const unsigned c = (T.first[T.tensors] + each - 1) / each; return c < 1u ? 1u : c < (unsigned)BLOCKS ? c : (unsigned)BLOCKS; }
 
 static int check_tensors(const char* who, int count, const int64_t* sizes, const void* const* grads, int dtype) {
     if (count <= 0 || !sizes || !grads) return fail(CKR_ERR_INVALID, "%s: no tensors", who);
@@ -321,7 +382,7 @@ int ckr_grad_norm(int32_t count, const int64_t* sizes, const void* const* grads,
             if (dtypes[k] < CKR_F32 || dtypes[k] > CKR_F16) return fail(CKR_ERR_INVALID, "ckr_grad_norm: unknown type %d", (int)dtypes[k]);
             TensorTable T;
             fill_table(T, end, k, sizes, nullptr, nullptr, grads);
-            const unsigned grid = grid_of(T);
+            const unsigned grid = grid_of(T, 4);
             if (pass) {
                 hipStream_t s = (hipStream_t)stream;
                 if (dtypes[k] == CKR_F32) hipLaunchKernelGGL((k_grad_norm<float>), dim3(grid), dim3(256), 0, s, T, max_norm, d_parts, (int)base, (int)total, d_ticket, d_out);

@@ -14,6 +14,7 @@ from . import _lib
 
 BLOCK = 128                         # elements that share a scale in 8-bit moments; every tensor's part of the states is padded to it
 TENSORS, BLOCKS = 96, 2048          # of one launch (ckr_adamw.hip)
+TICKET_WORDS = 1056                 # CKR_TICKET_WORDS
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # accessors for map(): a step looks at every parameter and gradient
 _SHAPE, _DTYPE, _GRAD = attrgetter("shape"), attrgetter("dtype"), attrgetter("grad")
@@ -122,7 +123,7 @@ class AdamW:
                 if p.dtype != torch.float32:
                     self._flat_view(self.master, p, o).copy_(p.detach())
         self.steps = z(max(1, first), torch.int32)                     # in the order of the batches
-        self._ticket = z(2, torch.int32)
+        self._ticket = z(2 * TICKET_WORDS, torch.int32)                # of the step, of the norm
         # partial sums of the norm: one launch for each run of up to TENSORS tensors of one type
         launches = sum((b.n + TENSORS - 1) // TENSORS for b in self._batches)
         self._parts, self._norm = (z(max(1, launches) * BLOCKS, torch.float64), z(2, torch.float64)) if self.max_norm is not None else (None, None)
@@ -211,7 +212,7 @@ class AdamW:
         p0, g0 = ps.buffer_info()[0], gs.buffer_info()[0]
         if self.max_norm is not None:
             _lib.check(L.ckr_grad_norm(len(gs), self._sizes_all, g0, self._dtypes_all, self.max_norm, self._parts.data_ptr(), self._parts.numel(),
-                                       self._ticket.data_ptr() + 4, self._norm.data_ptr(), s))
+                                       self._ticket.data_ptr() + 4 * TICKET_WORDS, self._norm.data_ptr(), s))
         for b in self._batches:
             lr, (b1, b2), eps, decay = b.seen
             on_device = isinstance(lr, torch.Tensor)

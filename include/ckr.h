@@ -750,8 +750,9 @@ int ckr_logprobs_backward(const ckr_logprobs_args* a, void* stream);
  * c = d_norm[1] (NULL: 1); lr = *d_lr, or lr where d_lr is NULL.  Parameters of 16 bits: w is the float32 master copy, the
  * parameter its rounding.  state_bits 32: m, v float32.  state_bits 8: bytes with a scale byte for each 128 elements
  * (m_scale, v_scale); m: sign, 4 exponent, 3 mantissa bits, v: 5 exponent, 3 mantissa bits, rounded stochastically with the bits of
- * Philox4x32-10 (key seed, counter (element / 8, t)).  d_ticket: a word that is 0 before the first call and not shared with
- * calls that may run at the same time. */
+ * Philox4x32-10 (key seed, counter (element / 8, t)).  d_ticket: CKR_TICKET_WORDS words that are 0 before the first call and not
+ * shared with calls that may run at the same time. */
+#define CKR_TICKET_WORDS 1056
 typedef struct {
     const int64_t* sizes; const int64_t* offsets; void* const* params; const void* const* grads;
     float* master; void* m; void* v; uint8_t* m_scale; uint8_t* v_scale;
