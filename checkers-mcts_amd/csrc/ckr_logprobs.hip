@@ -297,18 +297,20 @@ __global__ __launch_bounds__(64) void k_logprobs_join(const Args A, int parts) {
         join_lanes(s, c);
         TopList list;
         if constexpr (TOP) {                                                      // rank by rank: where no part's next one can enter, none behind it can
-            const long long at = row * parts * A.top;
-            for (int r = 0; r < A.top; ++r) {
-                bool any = false;
-                for (int p0 = 0; p0 < parts; p0 += 64) {
-                    const bool have = p0 + lane < parts;
-                    const float x = have ? tv[at + r * parts + p0 + lane] : -__builtin_huge_valf();
-                    if (!(list.tau > -__builtin_huge_valf())) list.bound_from_below(x, A.top);
-                    if (!__any(x >= list.tau && x > -__builtin_huge_valf())) continue;
-                    any = true;
-                    list.offer(x, have ? ti[at + r * parts + p0 + lane] : -1, A.top);
-                }
-                if (!any) break;
+            const int n = parts * A.top;
+            const float* v = tv + row * n;
+            const int* i = ti + row * n;
+            float x = lane < n ? v[lane] : -__builtin_huge_valf();
+            int j = lane < n ? i[lane] : -1, idle = 0;
+            for (int q = 0; q < n && idle < parts; q += 64) {
+                const int next = q + 64 + lane;
+                const float x1 = next < n ? v[next] : -__builtin_huge_valf();
+                const int j1 = next < n ? i[next] : -1;
+                if (!(list.tau > -__builtin_huge_valf())) list.bound_from_below(x, A.top);
+                const bool any = __any(x >= list.tau && x > -__builtin_huge_valf());
+                idle = any ? 0 : idle + 64;
+                if (any) list.offer(x, j, A.top);
+                x = x1; j = j1;
             }
         }
         write_row<T, MASK, TOP>(A, row, s, list);

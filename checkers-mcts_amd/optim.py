@@ -17,7 +17,7 @@ TENSORS, BLOCKS = 96, 2048          # of one launch (ckr_adamw.hip)
 TICKET_WORDS = 1056                 # CKR_TICKET_WORDS
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # accessors for map(): a step looks at every parameter and gradient
-_SHAPE, _DTYPE, _GRAD = attrgetter("shape"), attrgetter("dtype"), attrgetter("grad")
+_SHAPE, _DTYPE, _GRAD, _NBYTES = attrgetter("shape"), attrgetter("dtype"), attrgetter("grad"), attrgetter("nbytes")
 _STRIDE, _DEVICE, _POINTER = torch.Tensor.stride, torch.Tensor.get_device, torch.Tensor.data_ptr
 
 
@@ -131,8 +131,9 @@ class AdamW:
         self._sizes_all = (C.c_int64 * first)(*[p.numel() for p in self._every])
         self._dtypes_all = (C.c_int32 * first)(*[DTYPES[p.dtype] for p in self._every])
         self._layouts = [_layout(p) for p in self._every]
-        self._shape_of, self._stride_of, self._type_of = ([f(p) for p in self._every] for f in (_SHAPE, _STRIDE, _DTYPE))
+        self._shape_of, self._stride_of, self._type_of, self._nbytes_of = ([f(p) for p in self._every] for f in (_SHAPE, _STRIDE, _DTYPE, _NBYTES))
         self._device_of = [dev.index] * first
+        self._adopt()
         self._streams = {torch.cuda.current_stream(dev).cuda_stream}
         torch.cuda.current_stream(dev).synchronize()                   # a step on any stream finds the states in place
         self._L = _lib.load()
@@ -164,16 +165,27 @@ class AdamW:
     def _pointers(self):
         """Device addresses of all parameters and gradients in the order of the batches (0: no gradient), and copies of gradients that lie
         otherwise than their parameters."""
-        ps = self._every
-        if list(map(_SHAPE, ps)) != self._shape_of or list(map(_STRIDE, ps)) != self._stride_of or list(map(_DTYPE, ps)) != self._type_of \
-                or list(map(_DEVICE, ps)) != self._device_of:
-            raise ValueError("a parameter's shape, strides, type or device changed after the optimiser was made")
-        gs, keep = list(map(_GRAD, ps)), []
-        if any(g is None for g in gs) or list(map(_STRIDE, gs)) != self._stride_of or list(map(_SHAPE, gs)) != self._shape_of \
-                or list(map(_DTYPE, gs)) != self._type_of or list(map(_DEVICE, gs)) != self._device_of:
-            gs = [self._gradient(i, g, keep) for i, g in enumerate(gs)]
-            return array("Q", map(_POINTER, ps)), array("Q", (0 if g is None else g.data_ptr() for g in gs)), keep
-        return array("Q", map(_POINTER, ps)), array("Q", map(_POINTER, gs)), keep
+        ps, keep = self._every, []
+        addresses = list(map(_POINTER, ps))
+        if addresses != self._addresses:                               # (_aliases keep the memory: at the same address it is the same)
+            self._adopt()
+            addresses = self._addresses
+        gs = list(map(_GRAD, ps))
+        try:
+            if list(map(_STRIDE, gs)) == self._stride_of and list(map(_NBYTES, gs)) == self._nbytes_of and list(map(_DEVICE, gs)) == self._device_of:
+                return array("Q", addresses), array("Q", map(_POINTER, gs)), keep
+        except (TypeError, AttributeError, RuntimeError):              # None, or sparse
+            pass
+        gs = [self._gradient(i, g, keep) for i, g in enumerate(gs)]
+        return array("Q", addresses), array("Q", (0 if g is None else g.data_ptr() for g in gs)), keep
+
+    def _adopt(self):
+        """Takes the parameters' memory as it is now, if it is laid out as it was."""
+        for p, shape, stride, dtype in zip(self._every, self._shape_of, self._stride_of, self._type_of):
+            if p.shape != shape or p.stride() != stride or p.dtype != dtype or p.device != self.device:
+                raise ValueError("a parameter's shape, strides, type or device changed after the optimiser was made")
+        self._aliases = [p.detach() for p in self._every]
+        self._addresses = list(map(_POINTER, self._every))
 
     def _gradient(self, i, g, keep):
         if g is None:
@@ -183,11 +195,10 @@ class AdamW:
         if g.shape != self._shape_of[i] or g.dtype != self._type_of[i] or g.device != self.device:
             raise ValueError("a gradient must have its parameter's shape, type and device")
         if _layout(g) != self._layouts[i]:
-            g = torch.empty_strided(g.shape, self._stride_of[i], dtype=g.dtype, device=g.device).copy_(g)
+            g = torch.empty_strided(g.shape, self._stride_of[i], dtype=g.dtype, device=g.device).copy_(g.detach())
             keep.append(g)
         return g
 
-    @torch.no_grad()
     def step(self):
         """One update of every parameter that has a gradient."""
         if torch.cuda.current_device() != self.device.index:
