@@ -90,7 +90,7 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 struct TopList {
     float v = -__builtin_huge_valf();
     int i = -1;
-    // what a candidate has to beat: the entry of rank k - 1, or (an element has to equal it at least) a bound from below
+    // what a candidate has to come before: the entry of rank k - 1
     float tau = -__builtin_huge_valf();
     int tau_i = -1;
 
@@ -116,16 +116,37 @@ struct TopList {
             if (xl > tau || (xl == tau && jl < tau_i)) insert(xl, jl, k);
         }
     }
-    // While the list is not full: k of the lanes have a candidate >= the k-th largest of their maxima `t`, so what is below it is none.
-    __device__ __forceinline__ void bound_from_below(float t, int k) {
-        float x = -__builtin_huge_valf();
-        for (int r = 0; r < k; ++r) {
-            x = wave_max_f32(t);
-            if (!(x > -__builtin_huge_valf())) return;
-            const int l = first_lane(__ballot(t == x));
-            t = lane_id() == l ? -__builtin_huge_valf() : t;
+    // The list of the candidates (x, j) of lanes 0 .. n - 1, one each, where it is empty so far; the other lanes have none (-inf).  A lane's rank
+    // is the number of lanes before it, counted over n broadcasts that do not wait for each other, and the values go to the
+    // lanes of their ranks: 0.5 us whatever k is, where taking out the largest k times is 0.16 us each.
+    __device__ __forceinline__ void build(float x, int j, int k, int n) {
+        const bool have = x > -__builtin_huge_valf();
+        const int bits = __float_as_int(x + 0.0f);                                // (-0 as 0)
+        const unsigned hi = bits < 0 ? ~(unsigned)bits : (unsigned)bits | 0x80000000u, lo = ~(unsigned)j;
+        const unsigned long long key = (unsigned long long)hi << 32 | lo, mine = __ballot(have);
+        int rank = 0;
+        for (int l = 0; l < n; ++l) {
+            const unsigned long long other = (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)hi, l) << 32 | (unsigned)__builtin_amdgcn_readlane((int)lo, l);
+            rank += other > key ? 1 : 0;
         }
-        tau = x; tau_i = 0x7FFFFFFF;
+        const unsigned long long below = (1ull << lane_id()) - 1ull;
+        if (!have) rank = __popcll(mine) + __popcll(~mine & below);               // none: behind the others, in their own order
+        v = __int_as_float(__builtin_amdgcn_ds_permute(rank << 2, __float_as_int(x)));
+        i = __builtin_amdgcn_ds_permute(rank << 2, have ? j : -1);
+        const float kv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), k - 1));
+        if (kv > -__builtin_huge_valf()) { tau = kv; tau_i = __builtin_amdgcn_readlane(i, k - 1); }
+    }
+    // ... of M candidates a lane, in the order of their indexes j(0) < j(1) < ...
+    template <int M, typename J> __device__ __forceinline__ void build_of(const float (&x)[M], J j, int k, int n) {
+        float best = -__builtin_huge_valf();
+        int at = 0;
+#pragma unroll
+        for (int e = 0; e < M; ++e) best = fmaxf(best, x[e]);
+#pragma unroll
+        for (int e = M - 1; e >= 0; --e) at = x[e] == best ? e : at;
+        build(best, j(at), k, n);
+#pragma unroll
+        for (int e = 0; e < M; ++e) offer(at == e ? -__builtin_huge_valf() : x[e], j(e), k);
     }
 };
 
@@ -141,17 +162,16 @@ __device__ __forceinline__ void carry(Sums& s, float m, float c) {
     s.m = m;
 }
 
-// The alternatives of a part of one tile are taken from the registers.  Over several tiles the list holds vectors instead of elements (the
-// largest of each vector, and the vector's number): a tile is looked at again only if one of its vectors can still enter, and at the end
-// lane r reads the vector of rank r and offers its elements.  The k best elements are in the k best vectors: any other vector's best
-// element has k elements before it, of a larger value or, as vectors are numbered like their elements, of the same value and a lower index.
+// The list holds vectors first (the largest element of each, and the vector's number): a tile is looked at again only if one of its vectors can
+// still enter, and at the end lane r reads the vector of rank r for its elements.  The k best elements are in the k best vectors: any
+// other vector's best element has k elements before it, of a larger value or, as vectors are numbered like their elements, of the
+// same value and a lower index.
 template <typename T, int MASK, bool TOP>
 __device__ __forceinline__ void scan(const Args& A, long long row, int begin, int end, Sums& s, TopList& list) {
     constexpr int N = Vec<T>::N, U = PER_LANE / N;
     const T* x = static_cast<const T*>(A.logits) + row * A.row_stride;
     const int lane = lane_id(), k = A.top;
     const float c = A.inv_temperature * LOG2E;
-    const bool one = end - begin <= TILE;
     s.m = LOWEST; s.S = 0.0f; s.D = 0.0f;
     typename Vec<T>::type raw[U];
 #pragma unroll
@@ -184,29 +204,20 @@ __device__ __forceinline__ void scan(const Args& A, long long row, int begin, in
                 }
             }
         if constexpr (TOP) {
-            if (!(list.tau > -__builtin_huge_valf())) list.bound_from_below(tm, k);
-            if (one) {
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (u < left && __any(vm[u] >= list.tau)) {
-#pragma unroll
-                        for (int e = 0; e < N; ++e) list.offer(v[u * N + e], j0 + (u * 64 + lane) * N + e, k);
-                    }
-            } else if (__any(tm >= list.tau)) {
+            if (j0 == begin) list.build_of(vm, [&](int u) { return u * 64 + lane; }, k, 64);
+            else if (__any(tm >= list.tau)) {
 #pragma unroll
                 for (int u = 0; u < U; ++u) list.offer(vm[u], (j0 - begin) / N + u * 64 + lane, k);
             }
         }
     }
-    if (TOP && !one) {
+    if constexpr (TOP) {
         float e[N];
         const bool have = lane < k && list.i >= 0;
         const int j = have ? begin + list.i * N : 0, n = have ? end : 0;                         // (a lane without a vector: no element is below 0)
         values<T, MASK>(A, row, x, j, n, load_vec<T>(x, j, n), e);
         TopList best;
-        if (list.tau > -__builtin_huge_valf()) { best.tau = list.tau; best.tau_i = 0x7FFFFFFF; }
-#pragma unroll
-        for (int i = 0; i < N; ++i) best.offer(e[i], j + i, k);
+        best.build_of(e, [&](int i) { return j + i; }, k, k);
         list = best;
     }
 }
@@ -246,24 +257,17 @@ __device__ __forceinline__ void write_row(const Args& A, long long row, const Su
 // and lists go to the scratch memory for k_logprobs_join: float4 [rows][parts], values and indexes [rows][top][parts].
 template <typename T, int MASK, bool TOP>
 __global__ __launch_bounds__(256, 4) void k_logprobs(const Args A, int parts, int length) {
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    Sums s;
-    if (parts == 1) {
-        for (long long row = (long long)blockIdx.x * 4 + wave; row < A.n; row += 4ll * gridDim.x) {
-            TopList list;
-            scan<T, MASK, TOP>(A, row, 0, (int)A.v, s, list);
-            join_lanes(s, A.inv_temperature * LOG2E);
-            write_row<T, MASK, TOP>(A, row, s, list);
-        }
-        return;
-    }
-    const int part = (int)blockIdx.x * 4 + wave;
+    const int wave = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int part = parts == 1 ? 0 : wave, begin = part * length;
     if (part >= parts) return;
-    const int begin = part * length, end = (int)A.v - begin < length ? (int)A.v : begin + length;
-    for (long long row = blockIdx.y; row < A.n; row += gridDim.y) {
+    const int end = (int)A.v - begin < length ? (int)A.v : begin + length;
+    const long long step = parts == 1 ? 4ll * gridDim.x : gridDim.y;
+    for (long long row = parts == 1 ? wave : blockIdx.y; row < A.n; row += step) {
+        Sums s;
         TopList list;
         scan<T, MASK, TOP>(A, row, begin, end, s, list);
         join_lanes(s, A.inv_temperature * LOG2E);
+        if (parts == 1) { write_row<T, MASK, TOP>(A, row, s, list); continue; }
         const long long at = row * parts + part;
         float4* sums = static_cast<float4*>(A.scratch);
         if (lane_id() == 0) sums[at] = make_float4(s.m, s.S, s.D, 0.0f);
@@ -306,10 +310,12 @@ __global__ __launch_bounds__(64) void k_logprobs_join(const Args A, int parts) {
                 const int next = q + 64 + lane;
                 const float x1 = next < n ? v[next] : -__builtin_huge_valf();
                 const int j1 = next < n ? i[next] : -1;
-                if (!(list.tau > -__builtin_huge_valf())) list.bound_from_below(x, A.top);
-                const bool any = __any(x >= list.tau && x > -__builtin_huge_valf());
-                idle = any ? 0 : idle + 64;
-                if (any) list.offer(x, j, A.top);
+                if (q == 0) list.build(x, j, A.top, n < 64 ? n : 64);
+                else {
+                    const bool any = __any(x >= list.tau && x > -__builtin_huge_valf());
+                    idle = any ? 0 : idle + 64;
+                    if (any) list.offer(x, j, A.top);
+                }
                 x = x1; j = j1;
             }
         }
@@ -377,12 +383,12 @@ __global__ __launch_bounds__(256) void k_logprobs_bwd(const Args A) {
     }
 }
 
-// How many parts a row is cut into.  A wavefront per row fills the card from about WAVES rows on; below that a row's tiles are spread over
-// more wavefronts, and a second launch joins them.
-constexpr int WAVES = 4096;
+// How many parts a row is cut into.  A wavefront per row fills the card from about 2048 rows on; below that a row's tiles are spread over
+// more wavefronts, and a second launch joins them.  Wanted are 4096 of them, or half of that where each has to make a list of alternatives
+// (517 rows of 50001, fp16: sums alone 18.6 us at 4096 and 19.4 at 2048, with a list of 10 under a mask 42 + 6 us and 38 + 5 us).
 static void split(const Args& A, int& parts, int& length) {
-    const long long tiles = (A.v + TILE - 1) / TILE;
-    const long long want = A.n >= WAVES / 2 ? 1 : (WAVES + A.n - 1) / (A.n > 0 ? A.n : 1);
+    const long long tiles = (A.v + TILE - 1) / TILE, waves = A.top ? 2048 : 4096;
+    const long long want = A.n >= 2048 ? 1 : (waves + A.n - 1) / (A.n > 0 ? A.n : 1);
     const long long each = tiles <= want ? 1 : (tiles + want - 1) / want;         // tiles of a part
     parts = (int)((tiles + each - 1) / each);
     length = parts == 1 ? (int)A.v : (int)each * TILE;
