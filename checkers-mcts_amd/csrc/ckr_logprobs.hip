@@ -18,7 +18,8 @@ constexpr float LOWEST = -3.402823466e38f, LOG2E = 1.44269504088896340736f;
 typedef ckr_logprobs_args Args;
 
 constexpr float FLOOR = -1e30f;               // differences below it are that: exp is 0 anyway, and 0 x -inf would be NaN
-constexpr int PER_LANE = 32, TILE = 64 * PER_LANE;            // elements of a row that a wavefront holds in registers at a time
+// Elements of a row that a wavefront holds in registers at a time: 64 bytes a lane (and as many on their way).
+constexpr int tile_of(int type_size) { return 64 * 64 / type_size; }
 
 // 16 bytes of logits that start at any element
 template <typename T> struct Vec {
@@ -168,7 +169,7 @@ __device__ __forceinline__ void carry(Sums& s, float m, float c) {
 // same value and a lower index.
 template <typename T, int MASK, bool TOP>
 __device__ __forceinline__ void scan(const Args& A, long long row, int begin, int end, Sums& s, TopList& list) {
-    constexpr int N = Vec<T>::N, U = PER_LANE / N;
+    constexpr int N = Vec<T>::N, U = 4, PER_LANE = U * N, TILE = tile_of(sizeof(T));
     const T* x = static_cast<const T*>(A.logits) + row * A.row_stride;
     const int lane = lane_id(), k = A.top;
     const float c = A.inv_temperature * LOG2E;
@@ -387,11 +388,12 @@ __global__ __launch_bounds__(256) void k_logprobs_bwd(const Args A) {
 // more wavefronts, and a second launch joins them.  Wanted are 4096 of them, or half of that where each has to make a list of alternatives
 // (517 rows of 50001, fp16: sums alone 18.6 us at 4096 and 19.4 at 2048, with a list of 10 under a mask 42 + 6 us and 38 + 5 us).
 static void split(const Args& A, int& parts, int& length) {
-    const long long tiles = (A.v + TILE - 1) / TILE, waves = A.top ? 2048 : 4096;
+    const int tile = tile_of(A.dtype == CKR_F32 ? 4 : 2);
+    const long long tiles = (A.v + tile - 1) / tile, waves = A.top ? 2048 : 4096;
     const long long want = A.n >= 2048 ? 1 : (waves + A.n - 1) / (A.n > 0 ? A.n : 1);
     const long long each = tiles <= want ? 1 : (tiles + want - 1) / want;         // tiles of a part
     parts = (int)((tiles + each - 1) / each);
-    length = parts == 1 ? (int)A.v : (int)each * TILE;
+    length = parts == 1 ? (int)A.v : (int)each * tile;
 }
 
 template <typename T, int MASK, bool TOP> int forward_tmk(const Args& A, hipStream_t s) {

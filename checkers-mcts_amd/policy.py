@@ -34,9 +34,9 @@ def _ptr(t):
 
 
 @functools.lru_cache(maxsize=1024)
-def _scratch_bytes(n, v, top):
+def _scratch_bytes(n, v, top, dtype):
     """ckr_logprobs_scratch: a function of the sizes alone."""
-    bytes_ = _lib.load().ckr_logprobs_scratch(C.byref(LogprobsArgs(n=n, v=v, top=top, inv_temperature=1.0, logits=16)))
+    bytes_ = _lib.load().ckr_logprobs_scratch(C.byref(LogprobsArgs(n=n, v=v, top=top, dtype=dtype, inv_temperature=1.0, logits=16)))
     if bytes_ < 0:
         _lib.check(int(bytes_))
     return bytes_
@@ -62,7 +62,7 @@ def _forward(x, actions, mask, mask_kind, top, inv_temperature, want_stats):
     if top:
         top_action, top_logp = empty((n, top), dtype=torch.int64, device=dev), empty((n, top), dtype=f32, device=dev)
     stats = empty((n, 4), dtype=f32, device=dev) if want_stats else None
-    need = _scratch_bytes(n, v, top)
+    need = _scratch_bytes(n, v, top, DTYPES[x.dtype])
     scratch = empty(need, dtype=torch.uint8, device=dev) if need else None
     a = LogprobsArgs(x.data_ptr(), _ptr(actions), _ptr(mask), _ptr(logp), entropy.data_ptr(), _ptr(top_action), _ptr(top_logp), _ptr(stats),
                      None, None, None, _ptr(scratch), n, v, x.stride(0) if n > 1 else v, mask.stride(0) if mask is not None and mask.shape[0] > 1 else 0, 0, need,
