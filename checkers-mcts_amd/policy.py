@@ -33,6 +33,11 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _given(actions, n):
+    """Given actions a row."""
+    return 0 if actions is None or n == 0 else actions.numel() // n
+
+
 @functools.lru_cache(maxsize=1024)
 def _scratch_bytes(n, v, top, dtype):
     """ckr_logprobs_scratch: a function of the sizes alone."""
@@ -46,14 +51,16 @@ def _call(fn, args, device):
     """Launch on the current stream of `device`."""
     index = device.index
     if index == torch.cuda.current_device():
-        _lib.check(fn(C.byref(args), _lib.raw_stream(index)))
+        rc = fn(C.byref(args), _lib.raw_stream(index))
     else:
         with torch.cuda.device(device):
-            _lib.check(fn(C.byref(args), _lib.raw_stream(index)))
+            rc = fn(C.byref(args), _lib.raw_stream(index))
+    if rc:
+        _lib.check(rc)
 
 
 def _forward(x, actions, mask, mask_kind, top, inv_temperature, want_stats):
-    """x [n, v] (last dimension dense), actions [n, k] or None, mask [n or 1, ...] or None."""
+    """x [n, v] (last dimension dense), actions dense, k a row, or None, mask [n or 1, ...] or None; logp has the actions' shape."""
     (n, v), dev, f32 = x.shape, x.device, torch.float32
     empty = torch.empty
     logp = None if actions is None else empty(actions.shape, dtype=f32, device=dev)
@@ -66,7 +73,7 @@ def _forward(x, actions, mask, mask_kind, top, inv_temperature, want_stats):
     scratch = empty(need, dtype=torch.uint8, device=dev) if need else None
     a = LogprobsArgs(x.data_ptr(), _ptr(actions), _ptr(mask), _ptr(logp), entropy.data_ptr(), _ptr(top_action), _ptr(top_logp), _ptr(stats),
                      None, None, None, _ptr(scratch), n, v, x.stride(0) if n > 1 else v, mask.stride(0) if mask is not None and mask.shape[0] > 1 else 0, 0, need,
-                     DTYPES[x.dtype], mask_kind, 0 if actions is None else actions.element_size(), 0 if actions is None else actions.shape[1], top, inv_temperature)
+                     DTYPES[x.dtype], mask_kind, 0 if actions is None else actions.element_size(), _given(actions, n), top, inv_temperature)
     _call(_lib.load().ckr_logprobs_forward, a, dev)
     return logp, entropy, top_action, top_logp, stats
 
@@ -94,7 +101,7 @@ class _Logprobs(torch.autograd.Function):
         n, v = x.shape
         a = LogprobsArgs(x.data_ptr(), _ptr(actions), _ptr(mask), None, None, None, None, stats.data_ptr(), _ptr(g_logp), _ptr(g_entropy), grad.data_ptr(), None,
                          n, v, x.stride(0) if n > 1 else v, mask.stride(0) if mask is not None and mask.shape[0] > 1 else 0, v, 0,
-                         DTYPES[x.dtype], ctx.mask_kind, 0 if actions is None else actions.element_size(), 0 if actions is None else actions.shape[1], 0,
+                         DTYPES[x.dtype], ctx.mask_kind, 0 if actions is None else actions.element_size(), _given(actions, n), 0,
                          ctx.inv_temperature)
         _call(_lib.load().ckr_logprobs_backward, a, x.device)
         return (grad,) + (None,) * 5
@@ -114,7 +121,9 @@ def _check_mask(mask, lead, v, device):
         raise ValueError("mask must be a bool tensor [..., %d] (True: allowed) or the int32 [..., 8] legal-move words of rules.movegen" % v)
     if mask.dim() < 1 or mask.shape[-1] != width:
         raise ValueError("the mask's last dimension must be %d, got %s" % (width, list(mask.shape)))
-    if mask.shape[:-1].numel() == 1:
+    if mask.dim() == 2 and len(lead) == 1 and mask.shape[0] == lead[0]:
+        pass
+    elif mask.shape[:-1].numel() == 1:
         mask = mask.reshape(1, width)
     else:
         try:
@@ -162,8 +171,6 @@ def action_logprobs(logits, actions=None, mask=None, top=0, temperature=1.0):
         shape = actions.shape
         if shape != lead and (len(shape) != len(lead) + 1 or shape[:-1] != lead or not 1 <= shape[-1] <= MOST):
             raise ValueError("actions must have the shape %s or %s + [1 .. %d], got %s" % (list(lead), list(lead), MOST, list(shape)))
-        if len(shape) != 2 or shape == lead:
-            actions = actions.reshape(x.shape[0], 1 if shape == lead else shape[-1])
         actions = actions.contiguous()
     mask_kind = MASK_NONE
     if mask is not None:
@@ -176,8 +183,6 @@ def action_logprobs(logits, actions=None, mask=None, top=0, temperature=1.0):
         entropy = entropy.reshape(lead)
         if top:
             top_action, top_logp = top_action.reshape(lead + (top,)), top_logp.reshape(lead + (top,))
-    if logp is not None and logp.shape != shape:
-        logp = logp.reshape(shape)
     return ActionLogprobs(logp, entropy, top_action, top_logp)
 
 
