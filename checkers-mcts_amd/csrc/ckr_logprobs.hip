@@ -163,22 +163,65 @@ __device__ __forceinline__ void carry(Sums& s, float m, float c) {
     s.m = m;
 }
 
-// The list holds vectors first (the largest element of each, and the vector's number): a tile is looked at again only if one of its vectors can
-// still enter, and at the end lane r reads the vector of rank r for its elements.  The k best elements are in the k best vectors: any
-// other vector's best element has k elements before it, of a larger value or, as vectors are numbered like their elements, of the
-// same value and a lower index.
+// A lane's best vector so far (its largest element, and the vector's number in the part) and the largest element of its second best: nothing
+// in a tile waits for other lanes.
+struct Best {
+    float v = -__builtin_huge_valf(), second = -__builtin_huge_valf();
+    int i = -1;
+    __device__ __forceinline__ void take(float x, int j) {
+        second = __builtin_amdgcn_fmed3f(x, v, second);
+        i = x > v ? j : i;
+        v = fmaxf(v, x);
+    }
+};
+
+// The alternatives of a part.  The k best elements are in the k best vectors: any other vector's best element has k elements before it, of a
+// larger value or, as vectors are numbered like their elements, of the same value and a lower index.  The k best vectors are among the
+// lanes' best ones and the others of those lanes whose second best reaches the list (k^2 / 128 of them on average), which
+// the wavefront reads again unless it has them still (vm: the last tile's).  At the end lane r reads the vector of rank r for its elements.
+template <typename T, int MASK, int U>
+__device__ __forceinline__ void alternatives(const Args& A, long long row, const T* x, int begin, int end, const Best& mine, const float (&vm)[U], TopList& list) {
+    constexpr int N = Vec<T>::N;
+    const int lane = lane_id(), k = A.top, vectors = (end - begin + N - 1) / N;
+    TopList vecs;
+    vecs.build(mine.v, mine.i, k, 64);
+    if (vectors <= 64 * U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) vecs.offer(u * 64 + lane == mine.i ? -__builtin_huge_valf() : vm[u], u * 64 + lane, k);
+    } else for (unsigned long long more = __ballot(mine.second > vecs.tau || (mine.second == vecs.tau && mine.second > -__builtin_huge_valf() &&
+                                                                       !(mine.v == vecs.tau && mine.i >= vecs.tau_i))); more; more &= more - 1) {
+        const int l = first_lane(more), known = __builtin_amdgcn_readlane(mine.i, l);
+        for (int i0 = l; i0 < vectors; i0 += 64 * 64) {                           // lane l has the vectors l, l + 64, ...
+            const int i = i0 + lane * 64, j = begin + i * N;
+            const bool have = i < vectors && i != known;
+            float e[N], m = -__builtin_huge_valf();
+            values<T, MASK>(A, row, x, j, have ? end : 0, load_vec<T>(x, j, have ? end : 0), e);
+#pragma unroll
+            for (int q = 0; q < N; ++q) m = fmaxf(m, e[q]);
+            vecs.offer(m, i, k);
+        }
+    }
+    float e[N];
+    const bool have = lane < k && vecs.i >= 0;
+    const int j = have ? begin + vecs.i * N : 0;                                  // (a lane without a vector: no element is below 0)
+    values<T, MASK>(A, row, x, j, have ? end : 0, load_vec<T>(x, j, have ? end : 0), e);
+    list.build_of(e, [&](int i) { return j + i; }, k, k);
+}
+
 template <typename T, int MASK, bool TOP>
 __device__ __forceinline__ void scan(const Args& A, long long row, int begin, int end, Sums& s, TopList& list) {
     constexpr int N = Vec<T>::N, U = 4, PER_LANE = U * N, TILE = tile_of(sizeof(T));
     const T* x = static_cast<const T*>(A.logits) + row * A.row_stride;
-    const int lane = lane_id(), k = A.top;
+    const int lane = lane_id();
     const float c = A.inv_temperature * LOG2E;
+    Best best;
+    float vm[U];
     s.m = LOWEST; s.S = 0.0f; s.D = 0.0f;
     typename Vec<T>::type raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) raw[u] = load_vec<T>(x, begin + (u * 64 + lane) * N, end);
     for (int j0 = begin; j0 < end; j0 += TILE) {
-        float v[PER_LANE], vm[U], tm = -__builtin_huge_valf();
+        float v[PER_LANE], tm = -__builtin_huge_valf();
         const int left = (end - j0 + 64 * N - 1) / (64 * N);                      // vectors of this tile that hold anything
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -205,22 +248,11 @@ __device__ __forceinline__ void scan(const Args& A, long long row, int begin, in
                 }
             }
         if constexpr (TOP) {
-            if (j0 == begin) list.build_of(vm, [&](int u) { return u * 64 + lane; }, k, 64);
-            else if (__any(tm >= list.tau)) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) list.offer(vm[u], (j0 - begin) / N + u * 64 + lane, k);
-            }
+            for (int u = 0; u < U; ++u) best.take(vm[u], (j0 - begin) / N + u * 64 + lane);
         }
     }
-    if constexpr (TOP) {
-        float e[N];
-        const bool have = lane < k && list.i >= 0;
-        const int j = have ? begin + list.i * N : 0, n = have ? end : 0;                         // (a lane without a vector: no element is below 0)
-        values<T, MASK>(A, row, x, j, n, load_vec<T>(x, j, n), e);
-        TopList best;
-        best.build_of(e, [&](int i) { return j + i; }, k, k);
-        list = best;
-    }
+    if constexpr (TOP) alternatives<T, MASK, U>(A, row, x, begin, end, best, vm, list);
 }
 
 // the lanes' sums over one maximum
