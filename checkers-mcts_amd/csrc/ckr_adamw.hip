@@ -22,19 +22,24 @@
 
 namespace ckr {
 
-constexpr int TENSORS = 96;                   // of one launch: their pointers and sizes travel in the kernel's arguments (< 4 KB)
 constexpr int CHUNK = 2048;                   // elements of one tensor that a workgroup takes at a time: 256 threads x 8
 constexpr int BLOCKS = 2048;                  // at most (8 workgroups of 256 threads on each of 256 CUs)
 constexpr int M_TOP = 15, V_TOP = 31;
 
-struct TensorTable {
-    void* p[TENSORS];
-    const void* g[TENSORS];
-    long long n[TENSORS], off[TENSORS];
-    unsigned first[TENSORS + 1];              // chunks before tensor i
+// The tensors of one launch travel in the kernel's arguments (4 KB): the step takes 128 of them, the norm, which reads gradients only, 240.
+constexpr int STEP_TENSORS = 128, NORM_TENSORS = 240;
+template <int CAP, bool STEP> struct TensorTable {
+    static constexpr int MOST = CAP;
+    const void* g[CAP];
+    void* p[STEP ? CAP : 1];
+    unsigned block[STEP ? CAP : 1];           // of the states: the tensor's first block of 128
+    unsigned first[CAP + 1];                  // chunks before tensor i
+    uint16_t tail[CAP];                       // elements of its last chunk
     int tensors;
+    __device__ __forceinline__ long long size(int i) const { return (long long)(first[i + 1] - first[i] - 1) * CHUNK + tail[i]; }
 };
-static_assert(sizeof(TensorTable) <= 3600, "the table has to fit the kernel arguments beside the hyperparameters");
+typedef TensorTable<STEP_TENSORS, true> StepTable;
+typedef TensorTable<NORM_TENSORS, false> NormTable;
 
 struct Hyper {
     float* master; void* m; void* v; uint8_t* m_scale; uint8_t* v_scale;
@@ -47,11 +52,13 @@ struct Hyper {
 
 // The tensor that chunk c belongs to, from one load of the whole table: kernel arguments lie in host memory, and each step of a bisection
 // would wait for them anew.
-__device__ __forceinline__ int tensor_of(const TensorTable& T, unsigned c) {
-    static_assert(TENSORS <= 128, "two entries a lane");
-    const int lane = lane_id();
-    const unsigned a = T.first[min(lane, T.tensors)], b = T.first[min(lane + 64, T.tensors)];
-    const int n = __popcll(__ballot(lane < T.tensors && a <= c)) + __popcll(__ballot(lane + 64 < T.tensors && b <= c));
+template <typename Table> __device__ __forceinline__ int tensor_of(const Table& T, unsigned c) {
+    int n = 0;
+#pragma unroll
+    for (int q = 0; q < Table::MOST; q += 64) {
+        const int i = q + lane_id();
+        n += __popcll(__ballot(i < T.tensors && T.first[min(i, T.tensors)] <= c));
+    }
     return __builtin_amdgcn_readfirstlane(n - 1);
 }
 
@@ -145,7 +152,7 @@ __device__ __forceinline__ unsigned share(unsigned chunks, unsigned b) { return 
 
 // ---- the update: a thread has 8 consecutive elements, 16 lanes a block of 128 --------------------------------------------------------
 template <typename T, int BITS>
-__global__ __launch_bounds__(256) void k_adamw(const TensorTable tab, const Hyper H) {
+__global__ __launch_bounds__(256) void k_adamw(const StepTable tab, const Hyper H) {
     const double lr = H.d_lr ? (double)*H.d_lr : H.lr;
     const double c = H.norm ? H.norm[1] : 1.0;
     const float decay = (float)(1.0 - lr * H.weight_decay);
@@ -159,7 +166,7 @@ __global__ __launch_bounds__(256) void k_adamw(const TensorTable tab, const Hype
         const float rate = (float)(lr / bc1), rs = (float)(1.0 / sqrt(bc2));
         T* const p = static_cast<T*>(tab.p[i]);
         const T* const g = static_cast<const T*>(tab.g[i]);
-        const long long n = tab.n[i], off = tab.off[i];
+        const long long n = tab.size(i), off = (long long)tab.block[i] * 128;
         for (; ch < stop; ++ch) {
             const long long e0 = (long long)(ch - tab.first[i]) * CHUNK + threadIdx.x * 8, left = n - e0;
             const long long s0 = off + e0;                                        // of the states: whole blocks of 128
@@ -227,10 +234,17 @@ __global__ __launch_bounds__(256) void k_adamw(const TensorTable tab, const Hype
 }
 
 // ---- the global norm: every workgroup's sum of squares in parts[base + blockIdx], the last of all `total` workgroups adds them in order --
+__device__ __forceinline__ double workgroup_sum(double s, double* red) {          // 256 threads, in a fixed order; red: 4 doubles of LDS
+    s = wave_sum_f64(s);
+    if (lane_id() == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
 template <typename T>
-__global__ __launch_bounds__(256) void k_grad_norm(const TensorTable tab, double max_norm, double* __restrict__ parts, int base, int total,
+__global__ __launch_bounds__(256) void k_grad_norm(const NormTable tab, double max_norm, double* __restrict__ parts, int base, int total,
                                                    unsigned* __restrict__ ticket, double* __restrict__ out) {
-    __shared__ double red[256];
+    __shared__ double red[4];
     double s = 0.0;
     const unsigned chunks = tab.first[tab.tensors], end = share(chunks, blockIdx.x + 1);
     unsigned ch = share(chunks, blockIdx.x);
@@ -238,7 +252,7 @@ __global__ __launch_bounds__(256) void k_grad_norm(const TensorTable tab, double
         const unsigned stop = min(end, tab.first[i + 1]);
         if (ch >= stop) continue;
         const T* const g = static_cast<const T*>(tab.g[i]) + threadIdx.x * 8;
-        const long long n = tab.n[i] - threadIdx.x * 8;
+        const long long n = tab.size(i) - threadIdx.x * 8;
         while (ch < stop) {                                                       // four chunks' loads at a time
             float x[4][8];
 #pragma unroll
@@ -254,18 +268,14 @@ __global__ __launch_bounds__(256) void k_grad_norm(const TensorTable tab, double
         }
         ch = stop;
     }
-    red[threadIdx.x] = s;
-    __syncthreads();
-    for (int d = 128; d >= 1; d >>= 1) { if ((int)threadIdx.x < d) red[threadIdx.x] += red[threadIdx.x + d]; __syncthreads(); }
-    if (!threadIdx.x) __hip_atomic_store(parts + base + blockIdx.x, red[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s = workgroup_sum(s, red);
+    if (!threadIdx.x) __hip_atomic_store(parts + base + blockIdx.x, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (!arrives_last(ticket, (unsigned)base + blockIdx.x, (unsigned)total)) return;
     s = 0.0;
     for (int b = threadIdx.x; b < total; b += 256) s += __hip_atomic_load(parts + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    red[threadIdx.x] = s;
-    __syncthreads();
-    for (int d = 128; d >= 1; d >>= 1) { if ((int)threadIdx.x < d) red[threadIdx.x] += red[threadIdx.x + d]; __syncthreads(); }
+    s = workgroup_sum(s, red);
     if (threadIdx.x) return;
-    const double norm = sqrt(red[0]), c = max_norm / (norm + 1e-6);
+    const double norm = sqrt(s), c = max_norm / (norm + 1e-6);
     out[0] = norm;
     out[1] = c >= 1.0 ? 1.0 : c;                                                  // NaN stays NaN
 }
@@ -303,21 +313,27 @@ __global__ __launch_bounds__(256) void k_moments_write(const float* __restrict__
     }
 }
 
-// tensors [k, k + TENSORS) of the call
-static void fill_table(TensorTable& T, int count, int k, const int64_t* sizes, const int64_t* offsets, void* const* params, const void* const* grads) {
-    T.tensors = count - k < TENSORS ? count - k : TENSORS;
+// tensors [k, end) of the call, as many of them as the table takes
+template <int CAP, bool STEP>
+static void fill_table(TensorTable<CAP, STEP>& T, int end, int k, const int64_t* sizes, const int64_t* offsets, void* const* params, const void* const* grads) {
+    T.tensors = end - k < CAP ? end - k : CAP;
     unsigned chunks = 0;
     for (int i = 0; i < T.tensors; ++i) {
-        T.p[i] = params ? params[k + i] : nullptr;
         T.g[i] = grads[k + i];
-        T.n[i] = sizes[k + i];
-        T.off[i] = offsets ? offsets[k + i] : 0;
+        if (STEP) {
+            T.p[i] = params[k + i];
+            T.block[i] = (unsigned)(offsets[k + i] / 128);
+        }
         T.first[i] = chunks;
+        T.tail[i] = (uint16_t)((sizes[k + i] - 1) % CHUNK + 1);
         chunks += T.g[i] ? (unsigned)((sizes[k + i] + CHUNK - 1) / CHUNK) : 0u;
     }
     T.first[T.tensors] = chunks;
 }
-static unsigned grid_of(const TensorTable& T, unsigned each = 1) { const unsigned c = (T.first[T.tensors] + each - 1) / each; return c < 1u ? 1u : c < (unsigned)BLOCKS ? c : (unsigned)BLOCKS; }
+template <typename Table> static unsigned grid_of(const Table& T, unsigned each) {
+    const unsigned c = (T.first[T.tensors] + each - 1) / each;
+    return c < 1u ? 1u : c < (unsigned)BLOCKS ? c : (unsigned)BLOCKS;
+}
 
 static int check_tensors(const char* who, int count, const int64_t* sizes, const void* const* grads, int dtype) {
     if (count <= 0 || !sizes || !grads) return fail(CKR_ERR_INVALID, "%s: no tensors", who);
@@ -342,17 +358,18 @@ int ckr_adamw_step(const ckr_adamw_args* a, void* stream) {
     if (!(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0) || !(a->eps > 0.0f)) return fail(CKR_ERR_INVALID, "ckr_adamw_step: betas in [0, 1), eps > 0");
     for (int i = 0; i < a->count; ++i) {
         if (a->grads[i] && !a->params[i]) return fail(CKR_ERR_INVALID, "ckr_adamw_step: tensor %d has a gradient and no parameter", i);
-        if (a->offsets[i] < 0 || a->offsets[i] % 128) return fail(CKR_ERR_INVALID, "ckr_adamw_step: offsets are multiples of 128");
+        if (a->offsets[i] < 0 || a->offsets[i] % 128 || a->offsets[i] >> 38) return fail(CKR_ERR_INVALID, "ckr_adamw_step: offsets are multiples of 128 below 2^38");
     }
     if (int rc = require_device()) return rc;
     hipStream_t s = (hipStream_t)stream;
-    for (int k = 0; k < a->count; k += TENSORS) {
-        TensorTable T;
+    for (int k = 0; k < a->count; k += STEP_TENSORS) {
+        StepTable T;
         fill_table(T, a->count, k, a->sizes, a->offsets, a->params, a->grads);
         if (!T.first[T.tensors]) continue;
         const Hyper H = {a->master, a->m, a->v, a->m_scale, a->v_scale, a->d_step + k, a->d_ticket, a->d_lr, a->d_norm, a->lr, a->beta1, a->beta2,
                          std::log(a->beta1), std::log(a->beta2), a->weight_decay, (unsigned long long)a->seed, a->eps};
-        const dim3 grid(grid_of(T)), block(256);
+        static_assert(sizeof(T) + sizeof(H) <= 4096, "kernel arguments");
+        const dim3 grid(grid_of(T, 1)), block(256);
 #define CKR_ADAMW(TYPE)                                                                                       \
         do {                                                                                                  \
             if (a->state_bits == 32) hipLaunchKernelGGL((k_adamw<TYPE, 32>), grid, block, 0, s, T, H);         \
@@ -372,15 +389,15 @@ int ckr_grad_norm(int32_t count, const int64_t* sizes, const void* const* grads,
     using namespace ckr;
     if (int rc = check_tensors("ckr_grad_norm", count, sizes, grads, CKR_F32)) return rc;
     if (!dtypes || !d_parts || !d_ticket || !d_out || !(max_norm > 0.0)) return fail(CKR_ERR_INVALID, "ckr_grad_norm: bad argument");
-    // launches: runs of tensors of one type, at most TENSORS each
+    // launches: runs of tensors of one type, at most NORM_TENSORS each
     int64_t total = 0;
     for (int pass = 0; pass < 2; ++pass) {
         int64_t base = 0;
         for (int k = 0; k < count;) {
             int end = k;
-            while (end < count && end - k < TENSORS && dtypes[end] == dtypes[k]) ++end;
+            while (end < count && end - k < NORM_TENSORS && dtypes[end] == dtypes[k]) ++end;
             if (dtypes[k] < CKR_F32 || dtypes[k] > CKR_F16) return fail(CKR_ERR_INVALID, "ckr_grad_norm: unknown type %d", (int)dtypes[k]);
-            TensorTable T;
+            NormTable T;
             fill_table(T, end, k, sizes, nullptr, nullptr, grads);
             const unsigned grid = grid_of(T, 4);
             if (pass) {

@@ -417,11 +417,12 @@ __global__ __launch_bounds__(256) void k_logprobs_bwd(const Args A) {
 }
 
 // How many parts a row is cut into.  A wavefront per row fills the card from about 2048 rows on; below that a row's tiles are spread over
-// more wavefronts, and a second launch joins them.  Wanted are 4096 of them, or half of that where each has to make a list of alternatives
-// (517 rows of 50001, fp16: sums alone 18.6 us at 4096 and 19.4 at 2048, with a list of 10 under a mask 42 + 6 us and 38 + 5 us).
+// more wavefronts, and a second launch joins them.  Wanted are 6144 of them, or 2048 where each has to make a list of alternatives.
+// 517 rows of 50001, fp16, under a mask: sums alone 20.0 us at 6000 wavefronts, 23.8 at 4096; with a list of 10, 31.7 + 5.3 us at 2048, 33.4 + 6.3
+// at 4096.  1023 rows of 30011, float32: 22.6 and 24.8 us; with a list of 5, 26.9 and 34.7 us.
 static void split(const Args& A, int& parts, int& length) {
     const int tile = tile_of(A.dtype == CKR_F32 ? 4 : 2);
-    const long long tiles = (A.v + tile - 1) / tile, waves = A.top ? 2048 : 4096;
+    const long long tiles = (A.v + tile - 1) / tile, waves = A.top ? 2048 : 6144;
     const long long want = A.n >= 2048 ? 1 : (waves + A.n - 1) / (A.n > 0 ? A.n : 1);
     const long long each = tiles <= want ? 1 : (tiles + want - 1) / want;         // tiles of a part
     parts = (int)((tiles + each - 1) / each);

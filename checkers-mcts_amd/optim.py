@@ -13,7 +13,7 @@ import torch
 from . import _lib
 
 BLOCK = 128                         # elements that share a scale in 8-bit moments; every tensor's part of the states is padded to it
-TENSORS, BLOCKS = 96, 2048          # of one launch (ckr_adamw.hip)
+TENSORS, BLOCKS = 128, 2048         # of one launch (ckr_adamw.hip)
 TICKET_WORDS = 1056                 # CKR_TICKET_WORDS
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # accessors for map(): a step looks at every parameter and gradient

@@ -743,7 +743,7 @@ int ckr_logprobs_backward(const ckr_logprobs_args* a, void* stream);
 /* ---- AdamW over many tensors ---------------------------------------------------------------------------------------- *
  * Decoupled weight decay; the reference trains with Keras' Adam and l2 penalties (training_pipeline.py:49-114), which is
  * ckr_adam_step.  count tensors of one type: sizes[i] elements at params[i] / grads[i] (host arrays of device pointers; a NULL
- * gradient leaves its tensor, states and step number alone), states at element offsets[i] (a multiple of 128) of m, v and master,
+ * gradient leaves its tensor, states and step number alone), states at element offsets[i] (a multiple of 128 below 2^38) of m, v and master,
  * each tensor's part padded to whole blocks of 128.
  *     g = c grad;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  t = ++d_step[i]
  *     w = w (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
@@ -762,7 +762,7 @@ typedef struct {
 } ckr_adamw_args;
 int ckr_adamw_step(const ckr_adamw_args* a, void* stream);
 /* d_out[0] = sqrt of the sum of squares of all gradients (float64 sums in a fixed order), d_out[1] = min(1, max_norm / (d_out[0] +
- * 1e-6)).  d_parts: room for `parts` partial sums, 2048 for each run of up to 96 tensors of one type is enough. */
+ * 1e-6)).  d_parts: room for `parts` partial sums, 2048 for each run of up to 128 tensors of one type is enough. */
 int ckr_grad_norm(int32_t count, const int64_t* sizes, const void* const* grads, const int32_t* dtypes, double max_norm, double* d_parts,
                   int64_t parts, uint32_t* d_ticket, double* d_out, void* stream);
 /* 8-bit moments as float32 values, and float32 values as 8-bit moments (to the nearest code); n: a multiple of 128. */

@@ -84,7 +84,7 @@ def test_bad_arguments_of_adamw(lib, bad):
 def test_bad_arguments_of_the_norm_and_the_moments(lib):
     sizes, grads, kinds = (C.c_int64 * 2)(10, 10), (C.c_void_p * 2)(4096, 4096), (C.c_int32 * 2)(0, 0)
     good = [2, C.addressof(sizes), C.addressof(grads), C.addressof(kinds), 1.0, 4096, 4096, 4096, 4096, None]
-    for i, v in ((0, 0), (1, None), (2, None), (3, None), (4, 0.0), (4, -1.0), (4, float("nan")), (5, None), (6, 1), (7, None), (8, None)):
+    for i, v in ((0, 0), (1, None), (2, None), (3, None), (4, 0.0), (4, -1.0), (4, float("nan")), (5, None), (6, 0), (7, None), (8, None)):
         bad = list(good)
         bad[i] = v
         assert lib.ckr_grad_norm(*bad) == -1, i
