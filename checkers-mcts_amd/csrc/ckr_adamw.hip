@@ -124,8 +124,8 @@ __device__ __forceinline__ unsigned row16_max(unsigned v) {                     
 
 // ---- 8 consecutive elements of a thread, in 16-byte accesses that start at any element -------------------------------------------------
 template <typename T> struct Eight { typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T)))); };
-template <typename T> __device__ __forceinline__ void load8(const T* p, long long left, float* out) {       // left <= 0: none of them, zeros
-    if (left >= 8) {
+template <bool WHOLE, typename T> __device__ __forceinline__ void load8(const T* p, long long left, float* out) {       // left <= 0: none of them, zeros
+    if (WHOLE || left >= 8) {
         const typename Eight<T>::type v = *reinterpret_cast<const typename Eight<T>::type*>(p);
 #pragma unroll
         for (int j = 0; j < 8; ++j) out[j] = (float)v[j];
@@ -134,8 +134,8 @@ template <typename T> __device__ __forceinline__ void load8(const T* p, long lon
         for (int j = 0; j < 8; ++j) out[j] = j < left ? (float)p[j] : 0.0f;
     }
 }
-template <typename T> __device__ __forceinline__ void store8(T* p, long long left, const float* x) {
-    if (left >= 8) {
+template <bool WHOLE, typename T> __device__ __forceinline__ void store8(T* p, long long left, const float* x) {
+    if (WHOLE || left >= 8) {
         typename Eight<T>::type v;
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = (T)x[j];
@@ -151,80 +151,92 @@ template <typename T> __device__ __forceinline__ void store8(T* p, long long lef
 __device__ __forceinline__ unsigned share(unsigned chunks, unsigned b) { return (unsigned)((unsigned long long)chunks * b / gridDim.x); }
 
 // ---- the update: a thread has 8 consecutive elements, 16 lanes a block of 128 --------------------------------------------------------
+struct Factors { double c; float decay, rate, rs; int t; };      // of the gradient; 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t) of the weight
+
+// elements e0 .. e0 + 7 of a tensor of n, states at off + e0.  WHOLE: the chunk has all its elements; otherwise every access asks whether it has
+// (the question keeps the loads of a thread from being under way together).
+template <typename T, int BITS, bool WHOLE>
+__device__ __forceinline__ void update(const Hyper& H, const Factors& F, T* p, const T* g, long long e0, long long n, long long off) {
+    const long long left = n - e0, s0 = off + e0;
+    const bool in = WHOLE || e0 < (n + 127) / 128 * 128;                          // of the states: whole blocks of 128
+    float w[8], gr[8], mf[8], vf[8];
+    load8<WHOLE>(g + e0, left, gr);
+    if constexpr (sizeof(T) == 4) load8<WHOLE>(p + e0, left, w);
+    else load8<WHOLE>(H.master + s0, in ? 8 : 0, w);
+    if constexpr (BITS == 32) {
+        float* const m = static_cast<float*>(H.m) + s0;
+        float* const v = static_cast<float*>(H.v) + s0;
+        const float b1 = (float)H.beta1, b2 = (float)H.beta2, a1 = (float)(1.0 - H.beta1), a2 = (float)(1.0 - H.beta2), cf = (float)F.c;
+        load8<WHOLE>(m, in ? 8 : 0, mf);
+        load8<WHOLE>(v, in ? 8 : 0, vf);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float x = gr[j] * cf;
+            mf[j] = b1 * mf[j] + a1 * x;
+            vf[j] = b2 * vf[j] + a2 * x * x;
+        }
+        store8<WHOLE>(m, in ? 8 : 0, mf);
+        store8<WHOLE>(v, in ? 8 : 0, vf);
+    } else {
+        uint2* const m = reinterpret_cast<uint2*>(static_cast<uint8_t*>(H.m) + s0);
+        uint2* const v = reinterpret_cast<uint2*>(static_cast<uint8_t*>(H.v) + s0);
+        uint2 mc = make_uint2(0, 0), vc = make_uint2(0, 0);
+        int ms = 1, vs = 1;
+        if (in) { mc = *m; vc = *v; ms = H.m_scale[s0 / 128]; vs = H.v_scale[s0 / 128]; }
+        double md[8], vd[8];
+        unsigned hm = 0, hv = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const double x = (double)gr[j] * F.c;
+            md[j] = H.beta1 * decode_m(((j < 4 ? mc.x : mc.y) >> (8 * (j & 3))) & 255u, ms) + (1.0 - H.beta1) * x;
+            vd[j] = H.beta2 * decode_v(((j < 4 ? vc.x : vc.y) >> (8 * (j & 3))) & 255u, vs) + (1.0 - H.beta2) * x * x;
+            hm = max(hm, high_word(md[j])); hv = max(hv, high_word(vd[j]));
+            mf[j] = (float)md[j]; vf[j] = (float)vd[j];
+        }
+        const int ms1 = scale_byte(row16_max(hm)), vs1 = scale_byte(row16_max(hv));
+        const unsigned long long grp = (unsigned long long)s0 / 8;
+        const u32x4 r = philox((unsigned)H.seed, (unsigned)(H.seed >> 32), (unsigned)grp, (unsigned)(grp >> 32), (unsigned)F.t, 0u);
+        const unsigned rw[4] = {r.x, r.y, r.z, r.w};
+        unsigned mo[2] = {0, 0}, vo[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {                                             // 16 of 32 random bits for v, the others for m: 2 r + 1 of 2^17
+            const unsigned lo = rw[j >> 1] & 0xFFFFu, hi = rw[j >> 1] >> 16;
+            mo[j >> 2] |= encode_m(md[j], ms1, 2u * (j & 1 ? lo : hi) + 1u) << (8 * (j & 3));
+            vo[j >> 2] |= encode_v(vd[j], vs1, 2u * (j & 1 ? hi : lo) + 1u) << (8 * (j & 3));
+        }
+        if (in) {
+            *m = make_uint2(mo[0], mo[1]);
+            *v = make_uint2(vo[0], vo[1]);
+            if ((threadIdx.x & 15) == 0) { H.m_scale[s0 / 128] = (uint8_t)ms1; H.v_scale[s0 / 128] = (uint8_t)vs1; }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = w[j] * F.decay - F.rate * (mf[j] / (sqrtf(vf[j]) * F.rs + H.eps));
+    if constexpr (sizeof(T) != 4) store8<WHOLE>(H.master + s0, left < 8 ? left : 8, w);
+    store8<WHOLE>(p + e0, left, w);
+}
+
 template <typename T, int BITS>
 __global__ __launch_bounds__(256) void k_adamw(const StepTable tab, const Hyper H) {
     const double lr = H.d_lr ? (double)*H.d_lr : H.lr;
-    const double c = H.norm ? H.norm[1] : 1.0;
-    const float decay = (float)(1.0 - lr * H.weight_decay);
+    Factors F;
+    F.c = H.norm ? H.norm[1] : 1.0;
+    F.decay = (float)(1.0 - lr * H.weight_decay);
     const unsigned chunks = tab.first[tab.tensors], end = share(chunks, blockIdx.x + 1);
     unsigned ch = share(chunks, blockIdx.x);
     for (int i = tensor_of(tab, ch); ch < end; ++i) {                             // (tensors without a gradient have no chunks)
-        const unsigned stop = min(end, tab.first[i + 1]);
+        const unsigned begin = tab.first[i], after = tab.first[i + 1], stop = min(end, after);
         if (ch >= stop) continue;
-        const int t = H.step[i] + 1;
-        const double bc1 = -expm1(t * H.ln_beta1), bc2 = -expm1(t * H.ln_beta2);
-        const float rate = (float)(lr / bc1), rs = (float)(1.0 / sqrt(bc2));
+        F.t = H.step[i] + 1;
+        F.rate = (float)(lr / -expm1(F.t * H.ln_beta1));
+        F.rs = (float)(1.0 / sqrt(-expm1(F.t * H.ln_beta2)));
         T* const p = static_cast<T*>(tab.p[i]);
         const T* const g = static_cast<const T*>(tab.g[i]);
         const long long n = tab.size(i), off = (long long)tab.block[i] * 128;
         for (; ch < stop; ++ch) {
-            const long long e0 = (long long)(ch - tab.first[i]) * CHUNK + threadIdx.x * 8, left = n - e0;
-            const long long s0 = off + e0;                                        // of the states: whole blocks of 128
-            const bool in = e0 < (n + 127) / 128 * 128;
-            float w[8], gr[8], mf[8], vf[8];
-            load8(g + e0, left, gr);
-            if constexpr (sizeof(T) == 4) load8(p + e0, left, w);
-            else load8(H.master + s0, in ? 8 : 0, w);
-            if constexpr (BITS == 32) {
-                float* const m = static_cast<float*>(H.m) + s0;
-                float* const v = static_cast<float*>(H.v) + s0;
-                const float b1 = (float)H.beta1, b2 = (float)H.beta2, a1 = (float)(1.0 - H.beta1), a2 = (float)(1.0 - H.beta2), cf = (float)c;
-                load8(m, in ? 8 : 0, mf);
-                load8(v, in ? 8 : 0, vf);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float x = gr[j] * cf;
-                    mf[j] = b1 * mf[j] + a1 * x;
-                    vf[j] = b2 * vf[j] + a2 * x * x;
-                }
-                store8(m, in ? 8 : 0, mf);
-                store8(v, in ? 8 : 0, vf);
-            } else {
-                uint2* const m = reinterpret_cast<uint2*>(static_cast<uint8_t*>(H.m) + s0);
-                uint2* const v = reinterpret_cast<uint2*>(static_cast<uint8_t*>(H.v) + s0);
-                const uint2 mc = in ? *m : make_uint2(0, 0), vc = in ? *v : make_uint2(0, 0);
-                const int ms = in ? H.m_scale[s0 / 128] : 1, vs = in ? H.v_scale[s0 / 128] : 1;
-                double md[8], vd[8];
-                unsigned hm = 0, hv = 0;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const double x = (double)gr[j] * c;
-                    md[j] = H.beta1 * decode_m(((j < 4 ? mc.x : mc.y) >> (8 * (j & 3))) & 255u, ms) + (1.0 - H.beta1) * x;
-                    vd[j] = H.beta2 * decode_v(((j < 4 ? vc.x : vc.y) >> (8 * (j & 3))) & 255u, vs) + (1.0 - H.beta2) * x * x;
-                    hm = max(hm, high_word(md[j])); hv = max(hv, high_word(vd[j]));
-                    mf[j] = (float)md[j]; vf[j] = (float)vd[j];
-                }
-                const int ms1 = scale_byte(row16_max(hm)), vs1 = scale_byte(row16_max(hv));
-                const unsigned long long grp = (unsigned long long)s0 / 8;
-                const u32x4 r = philox((unsigned)H.seed, (unsigned)(H.seed >> 32), (unsigned)grp, (unsigned)(grp >> 32), (unsigned)t, 0u);
-                const unsigned rw[4] = {r.x, r.y, r.z, r.w};
-                unsigned mo[2] = {0, 0}, vo[2] = {0, 0};
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {                                     // 16 of 32 random bits for v, the others for m: 2 r + 1 of 2^17
-                    const unsigned lo = rw[j >> 1] & 0xFFFFu, hi = rw[j >> 1] >> 16;
-                    mo[j >> 2] |= encode_m(md[j], ms1, 2u * (j & 1 ? lo : hi) + 1u) << (8 * (j & 3));
-                    vo[j >> 2] |= encode_v(vd[j], vs1, 2u * (j & 1 ? hi : lo) + 1u) << (8 * (j & 3));
-                }
-                if (in) {
-                    *m = make_uint2(mo[0], mo[1]);
-                    *v = make_uint2(vo[0], vo[1]);
-                    if ((threadIdx.x & 15) == 0) { H.m_scale[s0 / 128] = (uint8_t)ms1; H.v_scale[s0 / 128] = (uint8_t)vs1; }
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = w[j] * decay - rate * (mf[j] / (sqrtf(vf[j]) * rs + H.eps));
-            if constexpr (sizeof(T) != 4) store8(H.master + s0, left < 8 ? left : 8, w);
-            store8(p + e0, left, w);
+            const long long e0 = (long long)(ch - begin) * CHUNK + threadIdx.x * 8;
+            if (ch + 1 < after || tab.tail[i] == CHUNK) update<T, BITS, true>(H, F, p, g, e0, n, off);
+            else update<T, BITS, false>(H, F, p, g, e0, n, off);
         }
     }
     // The workgroup that ends last advances the step counters: by then every other one has read them.
@@ -253,18 +265,26 @@ __global__ __launch_bounds__(256) void k_grad_norm(const NormTable tab, double m
         if (ch >= stop) continue;
         const T* const g = static_cast<const T*>(tab.g[i]) + threadIdx.x * 8;
         const long long n = tab.size(i) - threadIdx.x * 8;
+        const unsigned begin = tab.first[i], full = tab.first[i + 1] - (tab.tail[i] == CHUNK ? 0u : 1u);
         while (ch < stop) {                                                       // four chunks' loads at a time
+            const long long e0 = (long long)(ch - begin) * CHUNK;
             float x[4][8];
+            const unsigned take = ch + 4 <= min(stop, full) ? 4u : 1u;
+            if (take == 4u)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const long long e0 = (long long)(ch + q - tab.first[i]) * CHUNK;
-                load8(g + e0, ch + q < stop ? n - e0 : 0, x[q]);
+                for (int q = 0; q < 4; ++q) load8<true>(g + e0 + q * CHUNK, 8, x[q]);
+            else {
+                load8<false>(g + e0, n - e0, x[0]);
+#pragma unroll
+                for (int q = 1; q < 4; ++q)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[q][j] = 0.0f;
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) s = __builtin_fma((double)x[q][j], (double)x[q][j], s);
-            ch += 4;
+            ch += take;
         }
         ch = stop;
     }
@@ -292,8 +312,8 @@ __global__ __launch_bounds__(256) void k_moments_read(const uint8_t* __restrict_
             mo[j] = (float)decode_m(((j < 4 ? mc.x : mc.y) >> (8 * (j & 3))) & 255u, ms);
             vo[j] = (float)decode_v(((j < 4 ? vc.x : vc.y) >> (8 * (j & 3))) & 255u, vs);
         }
-        store8(m_out + i, 8, mo);
-        store8(v_out + i, 8, vo);
+        store8<true>(m_out + i, 8, mo);
+        store8<true>(v_out + i, 8, vo);
     }
 }
 __global__ __launch_bounds__(256) void k_moments_write(const float* __restrict__ m_in, const float* __restrict__ v_in, long long n, uint8_t* __restrict__ m,
