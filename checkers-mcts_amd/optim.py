@@ -81,7 +81,7 @@ class AdamW:
             g["params"] = [g["params"]] if isinstance(g["params"], torch.Tensor) else list(g["params"])
             for k, dflt in (("lr", lr), ("betas", betas), ("eps", eps), ("weight_decay", weight_decay)):
                 g.setdefault(k, dflt)
-        self.param_groups, self.state_bits, self.max_norm, self.seed = groups, int(state_bits), None if max_norm is None else float(max_norm), int(seed) & (2 ** 64 - 1)
+        self.param_groups, self.state_bits, self._max_norm, self.seed = groups, int(state_bits), None if max_norm is None else float(max_norm), int(seed) & (2 ** 64 - 1)
         every = [p for g in groups for p in g["params"]]
         if not every:
             raise ValueError("AdamW: no parameters")
@@ -95,9 +95,9 @@ class AdamW:
         spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in every if p.numel())
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("parameters share memory (or one is listed twice)")
+        self.device = dev = every[0].device
         for g in groups:
             self._check_group(g)
-        self.device = dev = every[0].device
         # the states: one flat buffer a moment, tensor i at offsets[i]
         self.params, self.offsets, total = every, [], 0
         for p in every:
@@ -119,14 +119,12 @@ class AdamW:
         self.master = None
         if any(p.dtype != torch.float32 for p in every):
             self.master = z(total, torch.float32)
-            for p, o in zip(every, self.offsets):
-                if p.dtype != torch.float32:
-                    self._flat_view(self.master, p, o).copy_(p.detach())
+            self.reset_master()
         self.steps = z(max(1, first), torch.int32)                     # in the order of the batches
         self._ticket = z(2 * TICKET_WORDS, torch.int32)                # of the step, of the norm
         # partial sums of the norm: one launch for each run of up to TENSORS tensors of one type
         launches = sum((b.n + TENSORS - 1) // TENSORS for b in self._batches)
-        self._parts, self._norm = (z(max(1, launches) * BLOCKS, torch.float64), z(2, torch.float64)) if self.max_norm is not None else (None, None)
+        self._parts, self._norm = (z(max(1, launches) * BLOCKS, torch.float64), z(2, torch.float64)) if self._max_norm is not None else (None, None)
         self._every = [p for b in self._batches for p in b.params]     # in the order of the batches
         self._sizes_all = (C.c_int64 * first)(*[p.numel() for p in self._every])
         self._dtypes_all = (C.c_int32 * first)(*[DTYPES[p.dtype] for p in self._every])
@@ -145,8 +143,8 @@ class AdamW:
     def _check_group(self, g):
         lr = g["lr"]
         if isinstance(lr, torch.Tensor):
-            if not lr.is_cuda or lr.dtype != torch.float32 or lr.numel() != 1:
-                raise ValueError("lr must be a number or a float32 device scalar")
+            if lr.device != self.device or lr.dtype != torch.float32 or lr.numel() != 1:
+                raise ValueError("lr must be a number or a float32 scalar on %s" % self.device)
         elif not 0 <= float(lr) < math.inf:
             raise ValueError("lr must be finite and not negative, got %r" % (lr,))
         b1, b2 = g["betas"]
@@ -221,8 +219,8 @@ class AdamW:
                 b.seen = now
         ps, gs, keep = self._pointers()
         p0, g0 = ps.buffer_info()[0], gs.buffer_info()[0]
-        if self.max_norm is not None:
-            _lib.check(L.ckr_grad_norm(len(gs), self._sizes_all, g0, self._dtypes_all, self.max_norm, self._parts.data_ptr(), self._parts.numel(),
+        if self._max_norm is not None:
+            _lib.check(L.ckr_grad_norm(len(gs), self._sizes_all, g0, self._dtypes_all, self._max_norm, self._parts.data_ptr(), self._parts.numel(),
                                        self._ticket.data_ptr() + 4 * TICKET_WORDS, self._norm.data_ptr(), s))
         for b in self._batches:
             lr, (b1, b2), eps, decay = b.seen
@@ -234,6 +232,10 @@ class AdamW:
         stepped = self._every if 0 not in gs else [p for p, g in zip(self._every, gs) if g]
         if stepped:
             torch.autograd.graph.increment_version(stepped)            # a backward pass over what it saved before the step is refused
+
+    @property
+    def max_norm(self):
+        return self._max_norm
 
     @property
     def grad_norm(self):
@@ -248,6 +250,14 @@ class AdamW:
         elif grads:
             with torch.no_grad():
                 torch._foreach_zero_(grads)
+
+    @torch.no_grad()
+    def reset_master(self):
+        """Takes the master copies from the 16-bit parameters: after something else than step() has changed them (load_state_dict() of the
+        module, say), which the next step would otherwise undo."""
+        for p, o in zip(self.params, self.offsets):
+            if p.dtype != torch.float32:
+                self._flat_view(self.master, p, o).copy_(p.detach())
 
     # ---- states ---------------------------------------------------------------------------------------------
     def moments(self):
@@ -297,7 +307,8 @@ class AdamW:
         self.steps.fill_(int(step))
 
     def state_dict(self):
-        """States (the buffers themselves) and hyperparameters; load_state_dict() of an optimiser over the same parameters takes it."""
+        """States (the buffers themselves) and hyperparameters; load_state_dict() of an optimiser over the same parameters takes it.  The
+        parameters are not among them, the master copies of 16-bit ones are."""
         return {"state_bits": self.state_bits, "seed": self.seed, "exp_avg": self.exp_avg, "exp_avg_sq": self.exp_avg_sq, "scales": self.scales,
                 "master": self.master, "steps": self.steps, "sizes": [p.numel() for p in self.params],
                 "param_groups": [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups]}

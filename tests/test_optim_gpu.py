@@ -492,6 +492,67 @@ def test_refusals():
         opt.step()
 
 
+def test_parameters_changed_otherwise_than_by_a_step():
+    from checkers_mcts_amd import optim
+    p = torch.ones(100, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    opt = optim.AdamW([p], lr=0.0)
+    p.grad = torch.zeros_like(p)
+    with torch.no_grad():
+        p.fill_(3.0)
+    opt.reset_master()
+    opt.step()
+    assert (p == 3).all() and (opt.master[:100] == 3).all()
+    # other memory of the same layout is taken over; the old one is left alone
+    q = torch.ones(100, device="cuda", requires_grad=True)
+    opt = optim.AdamW([q], lr=0.5, weight_decay=0.0, max_norm=1.0)
+    q.grad = torch.ones_like(q)
+    old = q.data
+    q.data = torch.full((100,), 5.0, device="cuda")
+    opt.step()
+    assert (old == 1).all() and (q < 5).all()
+    with pytest.raises(AttributeError):
+        opt.max_norm = 2.0
+    for change in (lambda t: t.half(), lambda t: t[:50], lambda t: t.cpu(), lambda t: t.reshape(10, 10)):
+        r = torch.ones(100, device="cuda", requires_grad=True)
+        opt = optim.AdamW([r])
+        r.grad = torch.ones_like(r)
+        r.data = change(r.data.clone())
+        with pytest.raises(ValueError):
+            opt.step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_offsets_beyond_32_bits(bits):
+    from checkers_mcts_amd import optim
+    n, lead = 2 ** 31 + 300, 200
+    small = torch.zeros(lead, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    p = torch.zeros(n, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    last = torch.ones(77, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    opt = optim.AdamW([small, p, last], lr=1e-2, state_bits=bits, max_norm=1e6, seed=3, weight_decay=0.0, eps=1e-6)
+    assert opt.offsets == [0, 256, 256 + (n + 127) // 128 * 128]
+    p.grad = torch.zeros_like(p)
+    g = torch.randn(5000, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").bfloat16()
+    p.grad[:5000] = g
+    p.grad[-5000:] = g
+    last.grad = g[:77].clone()
+    opt.step()
+    assert abs(float(opt.grad_norm) - math.sqrt(float(2 * g.double().square().sum() + g[:77].double().square().sum()))) <= 1e-9
+    x = g.double()
+    want = -0.01 * x / (x.abs() + 1e-6)
+    for part in (p[:5000], p[-5000:]):
+        assert float((part.detach().double() - want).abs().max()) <= 0.01 * 2.0 ** -8 * 1.01
+    assert (p[5000:-5000] == 0).all() and (small == 0).all() and opt.steps.tolist() == [0, 1, 1]
+    assert float((last.detach().double() - 1 - want[:77]).abs().max()) <= 2.0 ** -8 * 1.02
+    if bits == 8:
+        # the tensor's last whole block of 128, and the tensor behind it
+        at = 256 + n // 128 * 128 - 128
+        m, v = (t[at - (at - 256) % 128:][:128] for t in opt.moments())
+        block = p.grad[n // 128 * 128 - 128:n // 128 * 128].double()
+        rm, rv = dithers(3, at, 128, 1)
+        assert torch.equal(m, rounded((1 - 0.9) * block, 16, rm, False).float())
+        assert torch.equal(v, rounded((1 - 0.999) * block * block, 32, rv, True).float())
+
+
 def test_the_step_counts_as_a_change_in_place():
     from checkers_mcts_amd import optim
     p = torch.ones(10, device="cuda", requires_grad=True)

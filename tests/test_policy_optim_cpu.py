@@ -44,6 +44,17 @@ def test_missing_outputs_and_null_structures(lib):
     assert lib.ckr_logprobs_backward(C.byref(args(n_given=1)), None) == -1
 
 
+def test_scratch_memory_and_alignment(lib):
+    few = args(n=2, v=1 << 20, row_stride=1 << 20, top=3, top_action=4096, top_logp=4096)
+    need = lib.ckr_logprobs_scratch(C.byref(few))
+    assert need > 0 and lib.ckr_logprobs_scratch(C.byref(args(n=1 << 16, v=1 << 20))) == 0 and lib.ckr_logprobs_scratch(C.byref(args(v=1))) == 0
+    assert lib.ckr_logprobs_forward(C.byref(few), None) == -1 and b"scratch" in lib.ckr_last_error()
+    few.scratch, few.scratch_bytes = 4096, need - 1
+    assert lib.ckr_logprobs_forward(C.byref(few), None) == -1
+    for odd in (dict(stats=4100), dict(scratch=4104)):
+        assert lib.ckr_logprobs_forward(C.byref(args(**odd)), None) == -1
+
+
 def test_no_cpu_fallback(lib):
     if torch.cuda.is_available():
         pytest.skip("GPU present")
