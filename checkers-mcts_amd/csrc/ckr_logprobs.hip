@@ -7,6 +7,11 @@
 //     dx_j = it [ sum_k g_k [j = a_k] - p_j sum_k g_k - h p_j (log p_j + H) ]   (0 outside A)
 // Sums, statistics and outputs are float32; the gradient is rounded once, to the logits' type.
 // An empty A: log p = -inf, H = 0, no alternatives, gradient 0.  NaN or +inf in A: NaN, and no alternatives.
+//
+// What bounds it: the bytes of the logits.  Forward, 4096 x 32768 bf16: 52 us = 5.2 TB/s (a large copy reaches 4.7-5.4), with 5 alternatives
+// 58 us; 8192 x 16384 float32: 102 us = 5.2 TB/s.  Gradient, 4096 x 32768 bf16: 105 us = 5.1 TB/s read and written.  A single launch of
+// few rows is its chain of waits: one position (512) 5.5 us, 4096 positions 11 us (lists included), one row of 131072 with 20
+// alternatives 9 + 7 us.  Six VALU operations an element, one of them the exponential: at 7.5 TB/s they would be the bound.
 #include "ckr_host.h"
 #include "ckr_device.hip.h"
 #include <cmath>
@@ -177,8 +182,9 @@ struct Best {
 
 // The alternatives of a part.  The k best elements are in the k best vectors: any other vector's best element has k elements before it, of a
 // larger value or, as vectors are numbered like their elements, of the same value and a lower index.  The k best vectors are among the
-// lanes' best ones and the others of those lanes whose second best reaches the list (k^2 / 128 of them on average), which
-// the wavefront reads again unless it has them still (vm: the last tile's).  At the end lane r reads the vector of rank r for its elements.
+// lanes' best ones and the others of those lanes whose second best reaches the list (k^2 / 128 lanes on average; one that only equals
+// the list's last value lies 64 vectors behind the lane's best, if that equals it too), which the wavefront reads again unless
+// it has them still (vm: the last tile's).  At the end lane r reads the vector of rank r for its elements.
 template <typename T, int MASK, int U>
 __device__ __forceinline__ void alternatives(const Args& A, long long row, const T* x, int begin, int end, const Best& mine, const float (&vm)[U], TopList& list) {
     constexpr int N = Vec<T>::N;
@@ -189,7 +195,7 @@ __device__ __forceinline__ void alternatives(const Args& A, long long row, const
 #pragma unroll
         for (int u = 0; u < U; ++u) vecs.offer(u * 64 + lane == mine.i ? -__builtin_huge_valf() : vm[u], u * 64 + lane, k);
     } else for (unsigned long long more = __ballot(mine.second > vecs.tau || (mine.second == vecs.tau && mine.second > -__builtin_huge_valf() &&
-                                                                       !(mine.v == vecs.tau && mine.i >= vecs.tau_i))); more; more &= more - 1) {
+                                                                       !(mine.v == vecs.tau && mine.i + 64 >= vecs.tau_i))); more; more &= more - 1) {
         const int l = first_lane(more), known = __builtin_amdgcn_readlane(mine.i, l);
         for (int i0 = l; i0 < vectors; i0 += 64 * 64) {                           // lane l has the vectors l, l + 64, ...
             const int i = i0 + lane * 64, j = begin + i * N;
@@ -237,16 +243,18 @@ __device__ __forceinline__ void scan(const Args& A, long long row, int begin, in
 #pragma unroll
             for (int u = 0; u < U; ++u) raw[u] = load_vec<T>(x, j0 + TILE + (u * 64 + lane) * N, end);
         if (__any(tm > s.m)) carry(s, fmaxf(tm, s.m), c);
+        float S = 0.0f, D = 0.0f;                                                 // of the tile first: fewer roundings of the long sum
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (u < left) {
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
                     const float d = v[u * N + e] - s.m, p = exp2_fast(d * c);
-                    s.S += p;
-                    s.D = __builtin_fmaf(p, fmaxf(d, FLOOR), s.D);
+                    S += p;
+                    D = __builtin_fmaf(p, fmaxf(d, FLOOR), D);
                 }
             }
+        s.S += S; s.D += D;
         if constexpr (TOP) {
 #pragma unroll
             for (int u = 0; u < U; ++u) best.take(vm[u], (j0 - begin) / N + u * 64 + lane);
