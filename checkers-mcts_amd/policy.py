@@ -75,17 +75,22 @@ def _forward(x, actions, mask, mask_kind, top, inv_temperature, want_stats):
                      None, None, None, _ptr(scratch), n, v, x.stride(0) if n > 1 else v, mask.stride(0) if mask is not None and mask.shape[0] > 1 else 0, 0, need,
                      DTYPES[x.dtype], mask_kind, 0 if actions is None else actions.element_size(), _given(actions, n), top, inv_temperature)
     _call(_lib.load().ckr_logprobs_forward, a, dev)
-    return logp, entropy, top_action, top_logp, stats
+    return logp, entropy, top_action, top_logp, stats, a
+
+
+def _f32(g):
+    """An output's gradient as the kernel reads it (sums and means hand expanded ones down)."""
+    return g if g is None or (g.dtype is torch.float32 and g.is_contiguous()) else g.float().contiguous()
 
 
 class _Logprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, actions, mask, mask_kind, top, inv_temperature):
-        logp, entropy, top_action, top_logp, stats = _forward(x, actions, mask, mask_kind, top, inv_temperature, True)
+        logp, entropy, top_action, top_logp, stats, ctx.args = _forward(x, actions, mask, mask_kind, top, inv_temperature, True)
         ctx.save_for_backward(x, actions, mask, stats)
-        ctx.mask_kind, ctx.inv_temperature = mask_kind, inv_temperature
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(*(t for t in (top_action, top_logp) if t is not None))
+        if top:
+            ctx.mark_non_differentiable(top_action, top_logp)
         return logp, entropy, top_action, top_logp
 
     @staticmethod
@@ -94,15 +99,15 @@ class _Logprobs(torch.autograd.Function):
         if g_logp is None and g_entropy is None:
             return (None,) * 6
         x, actions, mask, stats = ctx.saved_tensors
-        if g_logp is None:
-            actions = None
         grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        g_logp, g_entropy = (None if g is None else g.float().contiguous() for g in (g_logp, g_entropy))
-        n, v = x.shape
-        a = LogprobsArgs(x.data_ptr(), _ptr(actions), _ptr(mask), None, None, None, None, stats.data_ptr(), _ptr(g_logp), _ptr(g_entropy), grad.data_ptr(), None,
-                         n, v, x.stride(0) if n > 1 else v, mask.stride(0) if mask is not None and mask.shape[0] > 1 else 0, v, 0,
-                         DTYPES[x.dtype], ctx.mask_kind, 0 if actions is None else actions.element_size(), _given(actions, n), 0,
-                         ctx.inv_temperature)
+        g_logp, g_entropy, a = _f32(g_logp), _f32(g_entropy), ctx.args
+        # the forward's arguments, with the tensors as they come back (hooks may have moved them)
+        a.logits, a.stats, a.grad, a.grad_stride, a.top = x.data_ptr(), stats.data_ptr(), grad.data_ptr(), x.shape[1], 0
+        a.row_stride = x.stride(0) if x.shape[0] > 1 else x.shape[1]
+        a.g_logp, a.g_entropy, a.actions, a.mask, a.scratch = _ptr(g_logp), _ptr(g_entropy), _ptr(actions), _ptr(mask), None
+        a.n_given = 0 if g_logp is None else _given(actions, x.shape[0])
+        if mask is not None:
+            a.mask_stride = mask.stride(0) if mask.shape[0] > 1 else 0
         _call(_lib.load().ckr_logprobs_backward, a, x.device)
         return (grad,) + (None,) * 5
 
@@ -178,7 +183,7 @@ def action_logprobs(logits, actions=None, mask=None, top=0, temperature=1.0):
     if x.requires_grad and torch.is_grad_enabled():
         logp, entropy, top_action, top_logp = _Logprobs.apply(x, actions, mask, mask_kind, top, 1.0 / temperature)
     else:
-        logp, entropy, top_action, top_logp, _ = _forward(x, actions, mask, mask_kind, top, 1.0 / temperature, False)
+        logp, entropy, top_action, top_logp = _forward(x, actions, mask, mask_kind, top, 1.0 / temperature, False)[:4]
     if len(lead) != 1:
         entropy = entropy.reshape(lead)
         if top:

@@ -373,6 +373,32 @@ def test_gradient_against_differences(v):
         assert abs(got - diff) <= 1e-6 * (1 + abs(diff)) + bound(v) * 30 * float((g.double().abs() * u.abs()).sum())
 
 
+def test_saved_tensors_that_come_back_elsewhere_and_two_backward_passes():
+    from checkers_mcts_amd import policy
+    x, a, allowed = make(40, 3000, torch.float32, 6, k=2)
+    a = a.clamp(min=0)
+    want = None
+    for hooks in (False, True):
+        leaf = x.clone().requires_grad_(True)
+        if hooks:
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
+                out = policy.action_logprobs(leaf, a, mask=allowed, top=3)
+        else:
+            out = policy.action_logprobs(leaf, a, mask=allowed, top=3)
+        g = torch.ones_like(out.logp.detach())
+        one, = torch.autograd.grad((out.logp, out.entropy), leaf, (g, torch.ones(40, device="cuda")), retain_graph=True)
+        two, = torch.autograd.grad(out.entropy.sum(), leaf, retain_graph=True)         # without the given actions, then with them again
+        three, = torch.autograd.grad((out.logp, out.entropy), leaf, (g, torch.ones(40, device="cuda")))
+        assert torch.equal(one, three) and not torch.equal(one, two)
+        want = want or (one, two)
+        assert torch.equal(one, want[0]) and torch.equal(two, want[1])
+    leaf = x.clone().requires_grad_(True)
+    out = policy.action_logprobs(leaf * 1.0, a, mask=allowed)
+    allowed.logical_not_()
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.entropy.sum().backward()
+
+
 def test_large_offsets():
     from checkers_mcts_amd import policy
     n, v = 66000, 32768                                                               # 2.16e9 logits: offsets beyond 32 bits
