@@ -8,10 +8,10 @@
 // Sums, statistics and outputs are float32; the gradient is rounded once, to the logits' type.
 // An empty A: log p = -inf, H = 0, no alternatives, gradient 0.  NaN or +inf in A: NaN, and no alternatives.
 //
-// What bounds it: the bytes of the logits.  Forward, 4096 x 32768 bf16: 52 us = 5.2 TB/s (a large copy reaches 4.7-5.4), with 5 alternatives
-// 58 us; 8192 x 16384 float32: 102 us = 5.2 TB/s.  Gradient, 4096 x 32768 bf16: 105 us = 5.1 TB/s read and written.  A single launch of
-// few rows is its chain of waits: one position (512) 5.5 us, 4096 positions 11 us (lists included), one row of 131072 with 20
-// alternatives 9 + 7 us.  Six VALU operations an element, one of them the exponential: at 7.5 TB/s they would be the bound.
+// What bounds it: the bytes of the logits.  Forward, 4096 x 32768 bf16: 47 us = 5.7 TB/s (a large copy reaches 4.7-5.4), with 5 alternatives
+// 54 us; 8192 x 16384 float32: 93 us = 5.8 TB/s.  Gradient, 4096 x 32768 bf16: 105 us = 5.1 TB/s read and written.  A single launch of
+// few rows is its chain of waits: one position (512) 5.5 us, 4096 positions 10 us (lists included), one row of 131072 with 20
+// alternatives 9.4 + 5.3 us.  Six VALU operations an element, one of them the exponential: at 7.5 TB/s they would be the bound.
 #include "ckr_host.h"
 #include "ckr_device.hip.h"
 #include <cmath>
@@ -23,9 +23,6 @@ constexpr float LOWEST = -3.402823466e38f, LOG2E = 1.44269504088896340736f;
 typedef ckr_logprobs_args Args;
 
 constexpr float FLOOR = -1e30f;               // differences below it are that: exp is 0 anyway, and 0 x -inf would be NaN
-// Elements of a row that a wavefront holds in registers at a time: 64 bytes a lane (and as many on their way).
-constexpr int tile_of(int type_size) { return 64 * 64 / type_size; }
-
 // 16 bytes of logits that start at any element
 template <typename T> struct Vec {
     static constexpr int N = 16 / sizeof(T);
@@ -169,35 +166,50 @@ __device__ __forceinline__ void carry(Sums& s, float m, float c) {
 }
 
 // A lane's best vector so far (its largest element, and the vector's number in the part) and the largest element of its second best: nothing
-// in a tile waits for other lanes.
+// in a tile waits for other lanes.  Lane l of every wavefront has the vectors l, l + 64, ..., so that lanes can be joined over wavefronts.
 struct Best {
     float v = -__builtin_huge_valf(), second = -__builtin_huge_valf();
     int i = -1;
-    __device__ __forceinline__ void take(float x, int j) {
+    __device__ __forceinline__ void take(float x, int j) {                        // j rises
         second = __builtin_amdgcn_fmed3f(x, v, second);
         i = x > v ? j : i;
         v = fmaxf(v, x);
     }
+    __device__ __forceinline__ void join(float v2, float second2, int i2) {
+        second = fmaxf(fminf(v, v2), fmaxf(second, second2));
+        i = v2 > v || (v2 == v && (unsigned)i2 < (unsigned)i) ? i2 : i;           // (-1, no vector, is the largest)
+        v = fmaxf(v, v2);
+    }
+};
+
+constexpr int GROUP = 4;                      // wavefronts of a workgroup
+constexpr int IN_TILE = 4;                    // vectors a lane holds at a time
+struct Shared {                               // what the wavefronts of a workgroup that share a part tell the first one
+    float vm[GROUP][IN_TILE][64];             // the vectors' largest elements, if each had one tile only
+    float v[GROUP][64], second[GROUP][64];
+    int i[GROUP][64];
+    float4 sums[GROUP];
 };
 
 // The alternatives of a part.  The k best elements are in the k best vectors: any other vector's best element has k elements before it, of a
 // larger value or, as vectors are numbered like their elements, of the same value and a lower index.  The k best vectors are among the
 // lanes' best ones and the others of those lanes whose second best reaches the list (k^2 / 128 lanes on average; one that only equals
 // the list's last value lies 64 vectors behind the lane's best, if that equals it too), which the wavefront reads again unless
-// it has them still (vm: the last tile's).  At the end lane r reads the vector of rank r for its elements.
-template <typename T, int MASK, int U>
-__device__ __forceinline__ void alternatives(const Args& A, long long row, const T* x, int begin, int end, const Best& mine, const float (&vm)[U], TopList& list) {
+// all are at hand (vm: `rows` times 64 of them, by `stride` wavefronts in turn).  At the end lane r reads the vector of rank r for its elements.
+template <typename T, int MASK>
+__device__ __forceinline__ void alternatives(const Args& A, long long row, int begin, int end, const Best& mine, const float (*vm)[IN_TILE][64], int stride, TopList& list) {
     constexpr int N = Vec<T>::N;
-    const int lane = lane_id(), k = A.top, vectors = (end - begin + N - 1) / N;
+    const T* x = static_cast<const T*>(A.logits) + row * A.row_stride;
+    const int lane = lane_id(), k = A.top, vectors = (end - begin + N - 1) / N, rows = (vectors + 63) / 64;
     TopList vecs;
     vecs.build(mine.v, mine.i, k, 64);
-    if (vectors <= 64 * U) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) vecs.offer(u * 64 + lane == mine.i ? -__builtin_huge_valf() : vm[u], u * 64 + lane, k);
+    if (rows <= IN_TILE * stride) {
+        for (int r = 0; r < rows; ++r)
+            vecs.offer(r * 64 + lane == mine.i ? -__builtin_huge_valf() : vm[r % stride][r / stride][lane], r * 64 + lane, k);
     } else for (unsigned long long more = __ballot(mine.second > vecs.tau || (mine.second == vecs.tau && mine.second > -__builtin_huge_valf() &&
                                                                        !(mine.v == vecs.tau && mine.i + 64 >= vecs.tau_i))); more; more &= more - 1) {
         const int l = first_lane(more), known = __builtin_amdgcn_readlane(mine.i, l);
-        for (int i0 = l; i0 < vectors; i0 += 64 * 64) {                           // lane l has the vectors l, l + 64, ...
+        for (int i0 = l; i0 < vectors; i0 += 64 * 64) {
             const int i = i0 + lane * 64, j = begin + i * N;
             const bool have = i < vectors && i != known;
             float e[N], m = -__builtin_huge_valf();
@@ -214,34 +226,34 @@ __device__ __forceinline__ void alternatives(const Args& A, long long row, const
     list.build_of(e, [&](int i) { return j + i; }, k, k);
 }
 
+// A wavefront's share of elements begin .. end - 1: the vectors of every `stride`-th 64, from the `first` 64 on.
 template <typename T, int MASK, bool TOP>
-__device__ __forceinline__ void scan(const Args& A, long long row, int begin, int end, Sums& s, TopList& list) {
-    constexpr int N = Vec<T>::N, U = 4, PER_LANE = U * N, TILE = tile_of(sizeof(T));
+__device__ __forceinline__ void scan(const Args& A, long long row, int begin, int end, int first, int stride, Sums& s, Best& best, float (*vm)[64]) {
+    constexpr int N = Vec<T>::N, U = IN_TILE, SPAN = 64 * N;
     const T* x = static_cast<const T*>(A.logits) + row * A.row_stride;
-    const int lane = lane_id();
+    const int lane = lane_id(), step = stride * SPAN;
     const float c = A.inv_temperature * LOG2E;
-    Best best;
-    float vm[U];
     s.m = LOWEST; s.S = 0.0f; s.D = 0.0f;
     typename Vec<T>::type raw[U];
+    int j0 = begin + first * SPAN;
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = load_vec<T>(x, begin + (u * 64 + lane) * N, end);
-    for (int j0 = begin; j0 < end; j0 += TILE) {
-        float v[PER_LANE], tm = -__builtin_huge_valf();
-        const int left = (end - j0 + 64 * N - 1) / (64 * N);                      // vectors of this tile that hold anything
+    for (int u = 0; u < U; ++u) raw[u] = load_vec<T>(x, j0 + u * step + lane * N, end);
+    for (; j0 < end; j0 += U * step) {
+        float v[U * N], m[U], tm = -__builtin_huge_valf();
+        const int left = (end - j0 + step - 1) / step;                            // vectors of this tile that hold anything
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            vm[u] = -__builtin_huge_valf();
+            m[u] = -__builtin_huge_valf();
             if (u < left) {
-                values<T, MASK>(A, row, x, j0 + (u * 64 + lane) * N, end, raw[u], v + u * N);
+                values<T, MASK>(A, row, x, j0 + u * step + lane * N, end, raw[u], v + u * N);
 #pragma unroll
-                for (int e = 0; e < N; ++e) vm[u] = fmaxf(vm[u], v[u * N + e]);
+                for (int e = 0; e < N; ++e) m[u] = fmaxf(m[u], v[u * N + e]);
             }
-            tm = fmaxf(tm, vm[u]);
+            tm = fmaxf(tm, m[u]);
         }
-        if (j0 + TILE < end)                                                      // the next tile is on its way while this one is summed
+        if (end - j0 > U * step)                                                  // the next tile is on its way while this one is summed
 #pragma unroll
-            for (int u = 0; u < U; ++u) raw[u] = load_vec<T>(x, j0 + TILE + (u * 64 + lane) * N, end);
+            for (int u = 0; u < U; ++u) raw[u] = load_vec<T>(x, j0 + (U + u) * step + lane * N, end);
         if (__any(tm > s.m)) carry(s, fmaxf(tm, s.m), c);
         float S = 0.0f, D = 0.0f;                                                 // of the tile first: fewer roundings of the long sum
 #pragma unroll
@@ -257,12 +269,20 @@ __device__ __forceinline__ void scan(const Args& A, long long row, int begin, in
         s.S += S; s.D += D;
         if constexpr (TOP) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) best.take(vm[u], (j0 - begin) / N + u * 64 + lane);
+            for (int u = 0; u < U; ++u) {
+                best.take(m[u], (j0 + u * step - begin) / N + lane);
+                vm[u][lane] = m[u];
+            }
         }
     }
-    if constexpr (TOP) alternatives<T, MASK, U>(A, row, x, begin, end, best, vm, list);
 }
 
+__device__ __forceinline__ void join_sums(Sums& s, Sums t, float c) {
+    const float m = fmaxf(s.m, t.m);
+    carry(s, m, c);
+    carry(t, m, c);
+    s.S += t.S; s.D += t.D;
+}
 // the lanes' sums over one maximum
 __device__ __forceinline__ void join_lanes(Sums& s, float c) {
     carry(s, wave_max_f32(s.m), c);
@@ -294,28 +314,49 @@ __device__ __forceinline__ void write_row(const Args& A, long long row, const Su
     }
 }
 
-// parts == 1: a wavefront per row.  Otherwise the row is cut into `parts` of `length` elements (whole tiles), a wavefront each, whose sums
-// and lists go to the scratch memory for k_logprobs_join: float4 [rows][parts], values and indexes [rows][top][parts].
-template <typename T, int MASK, bool TOP>
-__global__ __launch_bounds__(256, 4) void k_logprobs(const Args A, int parts, int length) {
-    const int wave = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int part = parts == 1 ? 0 : wave, begin = part * length;
-    if (part >= parts) return;
-    const int end = (int)A.v - begin < length ? (int)A.v : begin + length;
-    const long long step = parts == 1 ? 4ll * gridDim.x : gridDim.y;
-    for (long long row = parts == 1 ? wave : blockIdx.y; row < A.n; row += step) {
+// SHARE false: a wavefront per row.  SHARE true: a workgroup per part of a row, `parts` of `length` elements (whole 64 vectors) each; its first
+// wavefront joins the four and writes the row, or, if there are more parts, their sums and list to the scratch memory for
+// k_logprobs_join: float4 [rows][parts], values and indexes [rows][top][parts].
+template <typename T, int MASK, bool TOP, bool SHARE>
+__global__ __launch_bounds__(256, 4) void k_logprobs(const Args A, long long row0, int parts, int length) {
+    __shared__ Shared sh;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = lane_id();
+    const float c = A.inv_temperature * LOG2E;
+    if constexpr (!SHARE) {
+        const long long row = row0 + (long long)blockIdx.x * GROUP + wave;
+        if (row >= A.n) return;
         Sums s;
+        Best best;
         TopList list;
-        scan<T, MASK, TOP>(A, row, begin, end, s, list);
-        join_lanes(s, A.inv_temperature * LOG2E);
-        if (parts == 1) { write_row<T, MASK, TOP>(A, row, s, list); continue; }
+        scan<T, MASK, TOP>(A, row, 0, (int)A.v, 0, 1, s, best, sh.vm[wave]);
+        if constexpr (TOP) alternatives<T, MASK>(A, row, 0, (int)A.v, best, sh.vm + wave, 1, list);
+        join_lanes(s, c);
+        write_row<T, MASK, TOP>(A, row, s, list);
+    } else {
+        const long long row = row0 + (parts == 1 ? blockIdx.x : blockIdx.y);
+        const int part = parts == 1 ? 0 : (int)blockIdx.x, begin = part * length, end = (int)A.v - begin < length ? (int)A.v : begin + length;
+        Sums s;
+        Best best;
+        scan<T, MASK, TOP>(A, row, begin, end, wave, GROUP, s, best, sh.vm[wave]);
+        join_lanes(s, c);
+        if (wave && lane == 0) sh.sums[wave] = make_float4(s.m, s.S, s.D, 0.0f);
+        if (TOP && wave) { sh.v[wave][lane] = best.v; sh.second[wave][lane] = best.second; sh.i[wave][lane] = best.i; }
+        __syncthreads();
+        if (wave) return;
+        TopList list;
+        for (int w = 1; w < GROUP; ++w) {
+            join_sums(s, {sh.sums[w].x, sh.sums[w].y, sh.sums[w].z}, c);
+            if constexpr (TOP) best.join(sh.v[w][lane], sh.second[w][lane], sh.i[w][lane]);
+        }
+        if constexpr (TOP) alternatives<T, MASK>(A, row, begin, end, best, sh.vm, GROUP, list);
+        if (parts == 1) { write_row<T, MASK, TOP>(A, row, s, list); return; }
         const long long at = row * parts + part;
         float4* sums = static_cast<float4*>(A.scratch);
-        if (lane_id() == 0) sums[at] = make_float4(s.m, s.S, s.D, 0.0f);
-        if (TOP && lane_id() < A.top) {
+        if (lane == 0) sums[at] = make_float4(s.m, s.S, s.D, 0.0f);
+        if (TOP && lane < A.top) {
             float* tv = reinterpret_cast<float*>(sums + A.n * parts);
             int* ti = reinterpret_cast<int*>(tv + A.n * parts * A.top);
-            const long long slot = (row * A.top + lane_id()) * parts + part;
+            const long long slot = (row * A.top + lane) * parts + part;
             tv[slot] = list.v;
             ti[slot] = list.i;
         }
@@ -334,10 +375,7 @@ __global__ __launch_bounds__(64) void k_logprobs_join(const Args A, int parts) {
         for (int p = lane; p < parts; p += 64) {
             const float4 o = sums[row * parts + p];
             Sums t = {o.x, o.y, o.z};
-            const float m = fmaxf(s.m, t.m);
-            carry(s, m, c);
-            carry(t, m, c);
-            s.S += t.S; s.D += t.D;
+            join_sums(s, t, c);
         }
         join_lanes(s, c);
         TopList list;
@@ -424,28 +462,41 @@ __global__ __launch_bounds__(256) void k_logprobs_bwd(const Args A) {
     }
 }
 
-// How many parts a row is cut into.  A wavefront per row fills the card from about 2048 rows on; below that a row's tiles are spread over
-// more wavefronts, and a second launch joins them.  Wanted are 6144 of them, or 2048 where each has to make a list of alternatives.
-// 517 rows of 50001, fp16, under a mask: sums alone 20.0 us at 6000 wavefronts, 23.8 at 4096; with a list of 10, 31.7 + 5.3 us at 2048, 33.4 + 6.3
-// at 4096.  1023 rows of 30011, float32: 22.6 and 24.8 us; with a list of 5, 26.9 and 34.7 us.
-static void split(const Args& A, int& parts, int& length) {
-    const int tile = tile_of(A.dtype == CKR_F32 ? 4 : 2);
-    const long long tiles = (A.v + tile - 1) / tile, waves = A.top ? 2048 : 6144;
-    const long long want = A.n >= 2048 ? 1 : (waves + A.n - 1) / (A.n > 0 ? A.n : 1);
-    const long long each = tiles <= want ? 1 : (tiles + want - 1) / want;         // tiles of a part
-    parts = (int)((tiles + each - 1) / each);
-    length = parts == 1 ? (int)A.v : (int)each * tile;
+// How a row is shared.  A row of one tile is a wavefront's.  A longer one is a workgroup's if its wavefronts get two tiles each: one of four
+// makes the row's list while other workgroups read (4096 x 32768 bf16: 47 us, with 5 alternatives 54 us, against 52 and 58 us of a wavefront per
+// row; 8192 x 16384 float32: 93 and 102 us; but 16384 x 4096 bf16, half a tile each: 32 and 26 us), or if there are too few rows to
+// fill the card otherwise.  Rows fewer than about 1024 are cut into parts, which a second launch joins; where each has to make a list, a part
+// has a tile for each wavefront at least (one row of 131072 bf16 with 20 alternatives: 9.4 + 5.3 us for 16 parts, 8.6 + 7.2 us for 64; 517 rows of
+// 50001 fp16 under a mask with 10: 26.3 + 4.4 us at 1024 workgroups, 30.1 at 500, 27.7 + 5.4 us at 2560).
+static bool split(const Args& A, int& parts, int& length) {
+    constexpr long long GROUPS = 1024;
+    const int span = 64 * (A.dtype == CKR_F32 ? Vec<float>::N : Vec<_Float16>::N);                // 64 vectors
+    const long long n = A.n > 0 ? A.n : 1, rows = (A.v + span - 1) / span;
+    parts = 1;
+    length = (int)A.v;
+    if (rows <= IN_TILE || (n >= 2 * GROUPS && rows < 2 * IN_TILE * GROUP)) return false;
+    const long long want = n >= GROUPS ? 1 : (GROUPS + n / 2) / n, least = A.top ? GROUP * IN_TILE : GROUP;
+    const long long each = rows <= want * least ? least : (rows + want - 1) / want;
+    parts = (int)((rows + each - 1) / each);
+    length = parts == 1 ? (int)A.v : (int)each * span;
+    return true;
 }
 
 template <typename T, int MASK, bool TOP> int forward_tmk(const Args& A, hipStream_t s) {
     int parts, length;
-    split(A, parts, length);
-    const long long rows4 = (A.n + 3) / 4;
-    const dim3 grid = parts == 1 ? dim3((unsigned)(rows4 < (1 << 20) ? rows4 : 1 << 20)) : dim3((unsigned)((parts + 3) / 4), (unsigned)(A.n < 65535 ? A.n : 65535));
-    hipLaunchKernelGGL((k_logprobs<T, MASK, TOP>), grid, dim3(256), 0, s, A, parts, length);
-    CKR_HIP(hipGetLastError());
-    if (parts > 1) {
-        hipLaunchKernelGGL((k_logprobs_join<T, MASK, TOP>), dim3((unsigned)(A.n < (1 << 20) ? A.n : 1 << 20)), dim3(64), 0, s, A, parts);
+    const bool share = split(A, parts, length);
+    const long long most = 1 << 23, each = share ? most : most * GROUP;           // rows of a launch: a grid has less than 2^24 workgroups of this size
+    for (long long row0 = 0; row0 < A.n; row0 += each) {
+        const long long rows = A.n - row0 < each ? A.n - row0 : each;
+        if (!share)
+            hipLaunchKernelGGL((k_logprobs<T, MASK, TOP, false>), dim3((unsigned)((rows + GROUP - 1) / GROUP)), dim3(64 * GROUP), 0, s, A, row0, parts, length);
+        else if constexpr (MASK != CKR_MASK_LEGAL)                                // (512 actions are one tile)
+            hipLaunchKernelGGL((k_logprobs<T, MASK, TOP, true>), parts == 1 ? dim3((unsigned)rows) : dim3((unsigned)parts, (unsigned)rows), dim3(64 * GROUP), 0, s,
+                               A, row0, parts, length);
+        CKR_HIP(hipGetLastError());
+    }
+    if (parts > 1) {                                                              // (fewer than 1024 rows)
+        hipLaunchKernelGGL((k_logprobs_join<T, MASK, TOP>), dim3((unsigned)A.n), dim3(64), 0, s, A, parts);
         CKR_HIP(hipGetLastError());
     }
     return CKR_OK;

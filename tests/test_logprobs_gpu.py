@@ -419,6 +419,28 @@ def test_large_offsets():
     near(g[rows], want, size * (4 * bound(v) + 64 * U) + want.abs() * 2.0 ** -11 + 2.0 ** -25, "gradient")
 
 
+@pytest.mark.parametrize("n,v", [((1 << 25) + 9, 3), ((1 << 23) + 5, 16384 + 1)])
+def test_more_rows_than_a_launch_takes(n, v):
+    from checkers_mcts_amd import policy
+    row = torch.randn((v,), generator=torch.Generator(device="cuda").manual_seed(4), device="cuda").half()
+    a = torch.full((n,), 1, dtype=torch.int32, device="cuda")
+    out = policy.action_logprobs(row.expand(n, v), a, top=1)
+    one = reference(row[None], torch.ones((1, v), dtype=torch.bool, device="cuda"), torch.ones((1, 1), dtype=torch.long, device="cuda"), 1, 1.0)
+    assert bool((out.logp == out.logp[0]).all()) and bool((out.entropy == out.entropy[0]).all()) and bool((out.top_action == one[2][0, 0]).all())
+    near(out.logp[:1], one[0][0], bound(v) + 4 * U * one[0][0].abs() + 64 * U, "logp")
+    near(out.entropy[-1:], one[1], bound(v) * (1 + 2 * (one[1] + math.log(v))), "entropy")
+
+
+@pytest.mark.parametrize("n", [1, 3, 700, 1100, 2047, 2048, 2500])
+@pytest.mark.parametrize("v", [2049, 8193, 16384, 16500])
+def test_rows_shared_by_a_workgroup(n, v):
+    """Around the sizes at which a row goes from a wavefront to a workgroup and to several."""
+    x, a, allowed = make(n, v, torch.bfloat16, n + v, k=2)
+    check(x, allowed, allowed, a, top=7, grads=n < 1000, seed=v)
+    y = (x.float() / 8).round()                                                       # many ties
+    check(y, torch.ones_like(allowed), None, a, top=20, grads=False)
+
+
 def test_another_stream_and_two_calls_at_once():
     from checkers_mcts_amd import policy
     x, a, allowed = make(64, 20000, torch.float32, 2, k=2)
