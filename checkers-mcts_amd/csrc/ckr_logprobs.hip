@@ -119,10 +119,27 @@ struct TopList {
             if (xl > tau || (xl == tau && jl < tau_i)) insert(xl, jl, k);
         }
     }
-    // The list of the candidates (x, j) of lanes 0 .. n - 1, one each, where it is empty so far; the other lanes have none (-inf).  A lane's rank
-    // is the number of lanes before it, counted over n broadcasts that do not wait for each other, and the values go to the
-    // lanes of their ranks: 0.5 us whatever k is, where taking out the largest k times is 0.16 us each.
+    // The list of the candidates (x, j) of lanes 0 .. n - 1, one each, where it is empty so far; the other lanes have none (-inf).  Few ranks: the
+    // largest is taken out k times, 20 instructions that wait for each other.  Many: a lane's rank is the number of lanes before it,
+    // counted over n broadcasts that do not wait, and the values go to the lanes of their ranks, 350 instructions for 64.
     __device__ __forceinline__ void build(float x, int j, int k, int n) {
+        if (8 * k < n) {
+            for (int r = 0; r < k; ++r) {
+                const float best = wave_max_f32(x);
+                if (!(best > -__builtin_huge_valf())) return;
+                unsigned long long m = __ballot(x == best);
+                int l = first_lane(m), jl = __builtin_amdgcn_readlane(j, l);
+                for (m &= m - 1; m; m &= m - 1) {                                 // several: the lowest index
+                    const int l2 = first_lane(m), j2 = __builtin_amdgcn_readlane(j, l2);
+                    if (j2 < jl) { l = l2; jl = j2; }
+                }
+                v = lane_id() == r ? best : v;
+                i = lane_id() == r ? jl : i;
+                x = lane_id() == l ? -__builtin_huge_valf() : x;
+                if (r == k - 1) { tau = best; tau_i = jl; }
+            }
+            return;
+        }
         const bool have = x > -__builtin_huge_valf();
         const int bits = __float_as_int(x + 0.0f);                                // (-0 as 0)
         const unsigned hi = bits < 0 ? ~(unsigned)bits : (unsigned)bits | 0x80000000u, lo = ~(unsigned)j;
