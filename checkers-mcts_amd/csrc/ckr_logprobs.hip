@@ -9,9 +9,9 @@
 // An empty A: log p = -inf, H = 0, no alternatives, gradient 0.  NaN or +inf in A: NaN, and no alternatives.
 //
 // What bounds it: the bytes of the logits.  Forward, 4096 x 32768 bf16: 47 us = 5.7 TB/s (a large copy reaches 4.7-5.4), with 5 alternatives
-// 54 us; 8192 x 16384 float32: 93 us = 5.8 TB/s.  Gradient, 4096 x 32768 bf16: 105 us = 5.1 TB/s read and written.  A single launch of
-// few rows is its chain of waits: one position (512) 5.5 us, 4096 positions 10 us (lists included), one row of 131072 with 20
-// alternatives 9.4 + 5.3 us.  Six VALU operations an element, one of them the exponential: at 7.5 TB/s they would be the bound.
+// 52 us; 8192 x 16384 float32: 94 us = 5.7 TB/s.  Gradient, 4096 x 32768 bf16: 104 us = 5.2 TB/s read and written.  A launch of few or
+// short rows is a chain of waits: one position (512) 5.4 us, 4096 positions 4.6 us, 8 us with 5 alternatives, one row of 131072 with 20
+// alternatives 9.5 + 5.5 us.  Six VALU operations an element, one of them the exponential: at 7.5 TB/s they would be the bound.
 #include "ckr_host.h"
 #include "ckr_device.hip.h"
 #include <cmath>
@@ -481,7 +481,7 @@ __global__ __launch_bounds__(256) void k_logprobs_bwd(const Args A) {
 
 // How a row is shared.  A row of one tile is a wavefront's.  A longer one is a workgroup's if its wavefronts get two tiles each: one of four
 // makes the row's list while other workgroups read (4096 x 32768 bf16: 47 us, with 5 alternatives 54 us, against 52 and 58 us of a wavefront per
-// row; 8192 x 16384 float32: 93 and 102 us; but 16384 x 4096 bf16, half a tile each: 32 and 26 us), or if there are too few rows to
+// row, lists by ranks; 8192 x 16384 float32: 93 and 102 us; but 16384 x 4096 bf16, half a tile each: 32 and 26 us), or if there are too few rows to
 // fill the card otherwise.  Rows fewer than about 1024 are cut into parts, which a second launch joins; where each has to make a list, a part
 // has a tile for each wavefront at least (one row of 131072 bf16 with 20 alternatives: 9.4 + 5.3 us for 16 parts, 8.6 + 7.2 us for 64; 517 rows of
 // 50001 fp16 under a mask with 10: 26.3 + 4.4 us at 1024 workgroups, 30.1 at 500, 27.7 + 5.4 us at 2560).
