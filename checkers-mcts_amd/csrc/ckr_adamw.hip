@@ -307,20 +307,27 @@ __global__ __launch_bounds__(256) void k_grad_norm(const NormTable tab, double m
 }
 
 // ---- reading and writing 8-bit moments (n a multiple of 128) -------------------------------------------------------------------------
+// A lane has four elements at a time, so that a wavefront stores whole lines: 134 M in 215 us = 6.2 TB/s written and read, 280 us with
+// eight (half a line a store).
 __global__ __launch_bounds__(256) void k_moments_read(const uint8_t* __restrict__ m, const uint8_t* __restrict__ v, const uint8_t* __restrict__ m_scale,
                                                       const uint8_t* __restrict__ v_scale, long long n, float* __restrict__ m_out, float* __restrict__ v_out) {
-    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (long long)gridDim.x * 2048) {
-        const uint2 mc = *reinterpret_cast<const uint2*>(m + i), vc = *reinterpret_cast<const uint2*>(v + i);
-        const int ms = m_scale[i / 128], vs = v_scale[i / 128];
-        float mo[8], vo[8];
+    typedef float four __attribute__((ext_vector_type(4), aligned(4)));
+    for (long long i0 = (long long)blockIdx.x * 2048 + threadIdx.x * 4; i0 < n; i0 += (long long)gridDim.x * 2048)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            mo[j] = (float)decode_m(((j < 4 ? mc.x : mc.y) >> (8 * (j & 3))) & 255u, ms);
-            vo[j] = (float)decode_v(((j < 4 ? vc.x : vc.y) >> (8 * (j & 3))) & 255u, vs);
+        for (int q = 0; q < 2; ++q) {
+            const long long i = i0 + q * 1024;
+            if (i >= n) break;
+            const unsigned mc = *reinterpret_cast<const unsigned*>(m + i), vc = *reinterpret_cast<const unsigned*>(v + i);
+            const int ms = m_scale[i / 128], vs = v_scale[i / 128];
+            four mo, vo;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                mo[j] = (float)decode_m((mc >> (8 * j)) & 255u, ms);
+                vo[j] = (float)decode_v((vc >> (8 * j)) & 255u, vs);
+            }
+            *reinterpret_cast<four*>(m_out + i) = mo;
+            *reinterpret_cast<four*>(v_out + i) = vo;
         }
-        store8<true>(m_out + i, 8, mo);
-        store8<true>(v_out + i, 8, vo);
-    }
 }
 __global__ __launch_bounds__(256) void k_moments_write(const float* __restrict__ m_in, const float* __restrict__ v_in, long long n, uint8_t* __restrict__ m,
                                                        uint8_t* __restrict__ v, uint8_t* __restrict__ m_scale, uint8_t* __restrict__ v_scale) {

@@ -441,6 +441,13 @@ def test_rows_shared_by_a_workgroup(n, v):
     check(y, torch.ones_like(allowed), None, a, top=20, grads=False)
 
 
+@pytest.mark.parametrize("n,v,dtype,masked", [(2557, 16411, torch.float32, True), (2555, 16411, torch.float32, False), (2600, 32771, torch.bfloat16, False)], ids=str)
+def test_gradients_on_both_sides_of_the_caches(n, v, dtype, masked):
+    """Around 160 MiB, from which on they are stored past the caches."""
+    x, a, allowed = make(n, v, dtype, n, k=2)
+    check(x, allowed if masked else torch.ones_like(allowed), allowed if masked else None, a, seed=n)
+
+
 def test_another_stream_and_two_calls_at_once():
     from checkers_mcts_amd import policy
     x, a, allowed = make(64, 20000, torch.float32, 2, k=2)
