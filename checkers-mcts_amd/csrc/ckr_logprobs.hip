@@ -422,10 +422,6 @@ __global__ __launch_bounds__(64) void k_logprobs_join(const Args A, int parts) {
 // ---- backward: a wavefront has BWD_PER_LANE elements a lane of one row ----------------------------------------------------------------
 constexpr int BWD_PER_LANE = 16, BWD_TILE = 64 * BWD_PER_LANE;
 // A gradient of this many bytes is stored past the caches (STREAMS), which keep no more than its end for whoever reads it.  Forward, backward and
-// a reduction of the gradient, bf16 rows of 32768, with the caches and past them: 128 MB 129 and 152 us, 160 MB 189 and 185 us, 206 MB 247
-// and 237 us, 256 MB 313 and 291 us.
-constexpr long long STREAMED = 160ll << 20;
-// A gradient of this many bytes is stored past the caches (STREAMS), which keep no more than its end for whoever reads it.  Forward, backward and
 // a reduction of the gradient, bf16 rows of 32768, with the caches and past them: 128 MiB 129 and 152 us, 160 MiB 189 and 185 us, 206 MiB 247
 // and 237 us, 256 MiB 313 and 291 us.
 constexpr long long STREAMED = 160ll << 20;
