@@ -59,7 +59,8 @@ class AdamW:
 
     params        tensors, or groups {"params": [...], "lr": ..., "betas": ..., "eps": ..., "weight_decay": ...}, of float32, bfloat16
                   or float16 on one GPU, dense in memory (any order of dimensions).  16-bit parameters get a float32 master copy, which is
-                  what the optimiser updates; the parameter is its rounding.
+                  what the optimiser updates; the parameter is its rounding.  Their memory may be replaced (p.data = ...) by some of the same
+                  shape, strides and type.
     lr            a number, or a float32 device scalar (read by the kernel: a captured step follows its changes).
     state_bits    32, or 8: a byte for each moment and a scale byte for each 128 elements, rounded stochastically (seed).
     max_norm      clip the gradients by their global norm (over all groups): g * min(1, max_norm / (norm + 1e-6)); the norm of the last
@@ -174,6 +175,8 @@ class AdamW:
                 return array("Q", addresses), array("Q", map(_POINTER, gs)), keep
         except (TypeError, AttributeError, RuntimeError):              # None, or sparse
             pass
+        if list(map(_STRIDE, ps)) != self._stride_of:                  # the same memory, seen otherwise
+            self._adopt()
         gs = [self._gradient(i, g, keep) for i, g in enumerate(gs)]
         return array("Q", addresses), array("Q", (0 if g is None else g.data_ptr() for g in gs)), keep
 

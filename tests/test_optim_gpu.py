@@ -521,6 +521,18 @@ def test_parameters_changed_otherwise_than_by_a_step():
             opt.step()
 
 
+def test_the_same_memory_in_another_order_is_refused():
+    from checkers_mcts_amd import optim
+    p = torch.ones((8, 8), device="cuda", requires_grad=True)
+    opt = optim.AdamW([p])
+    p.data = p.data.t()
+    p.grad = torch.ones_like(p)
+    assert p.grad.stride() == p.stride() == (1, 8)
+    with pytest.raises(ValueError):
+        opt.step()
+    assert (p == 1).all() and int(opt.steps[0]) == 0
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_offsets_beyond_32_bits(bits):
     from checkers_mcts_amd import optim
