@@ -17,7 +17,7 @@
 // by the order of float32 operations (a v_fma_f64 issues at the rate of a v_fma_f32 here).
 // The price of so few bits is noise: v fluctuates by about 20 % around its average, its root, which divides, by 10 %.
 //
-// What bounds it: memory.  134 M bf16 parameters with master copies and 8-bit moments: 442 us = 4.9 TB/s (a large copy reaches 4.7-5.4); with 32-bit
+// What bounds it: memory.  134 M bf16 parameters with master copies and 8-bit moments: 440 us = 4.9 TB/s (a large copy reaches 4.7-5.4); with 32-bit
 // moments 9 M float16 in 170 tensors: 51 us = 4.9 TB/s; the 48 tensors of the policy / value network (1.3 M float32): 11 us, of which a
 // launch, the table and the tickets are 5.  In 8 bits the 90 VALU operations an element (20 of them Philox, shared by 8 elements) would
 // allow 7 TB/s.
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(256) void k_grad_norm(const NormTable tab, double m
 }
 
 // ---- reading and writing 8-bit moments (n a multiple of 128) -------------------------------------------------------------------------
-// A lane has four elements at a time, so that a wavefront stores whole lines: 134 M in 215 us = 6.2 TB/s written and read, 280 us with
+// A lane has four elements at a time, so that a wavefront stores whole lines: 134 M in 215-235 us = 5.7-6.2 TB/s written and read, 280 us with
 // eight (half a line a store).
 __global__ __launch_bounds__(256) void k_moments_read(const uint8_t* __restrict__ m, const uint8_t* __restrict__ v, const uint8_t* __restrict__ m_scale,
                                                       const uint8_t* __restrict__ v_scale, long long n, float* __restrict__ m_out, float* __restrict__ v_out) {

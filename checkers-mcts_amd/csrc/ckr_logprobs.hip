@@ -9,7 +9,7 @@
 // An empty A: log p = -inf, H = 0, no alternatives, gradient 0.  NaN or +inf in A: NaN, and no alternatives.
 //
 // What bounds it: the bytes of the logits.  Forward, 4096 x 32768 bf16: 47 us = 5.7 TB/s (a large copy reaches 4.7-5.4), with 5 alternatives
-// 52 us; 8192 x 16384 float32: 94 us = 5.7 TB/s.  Gradient, 4096 x 32768 bf16: 104 us = 5.2 TB/s read and written.  A launch of few or
+// 52 us; 8192 x 16384 float32: 94 us = 5.7 TB/s.  Gradient, 4096 x 32768 bf16: 96 us = 5.6 TB/s read and written.  A launch of few or
 // short rows is a chain of waits: one position (512) 5.4 us, 4096 positions 4.6 us, 8 us with 5 alternatives, one row of 131072 with 20
 // alternatives 9.5 + 5.5 us.  Six VALU operations an element, one of them the exponential: at 7.5 TB/s they would be the bound.
 #include "ckr_host.h"
