@@ -253,12 +253,16 @@ def losses(net, x, pi, tv, autocast_dtype=None, with_penalty=True, entropy_weigh
 
 
 @torch.no_grad()
-def policy_figures(net, x, pi):
-    """Sums over a batch (float64 [3]): the policy's entropy, the log probability of the most visited move, and how often that move is
-    among the network's three best -- all over the legal moves."""
-    move = pi.argmax(dim=1)
-    out = policy.action_logprobs(net.logits(x.permute(0, 3, 1, 2))[0], move, mask=policy.legal_from_features(x), top=3)
-    return torch.stack([out.entropy.double().sum(), out.logp.double().sum(), (out.top_action == move[:, None]).sum().double()])
+def policy_figures(net, x, pi, autocast_dtype=None):
+    """Sums over a batch (float64 [4]): the policy's entropy, the log probability of the most visited move, how often that move is
+    among the network's three best -- all over the legal moves -- and the rows that count.  A row without visits does not: a game that runs
+    to its end leaves one, whose position has no legal move.  autocast_dtype: as in `losses`."""
+    played, move = (pi > 0).any(dim=1), pi.argmax(dim=1)
+    with torch.autocast(device_type=x.device.type, dtype=autocast_dtype or torch.bfloat16, enabled=autocast_dtype not in (None, torch.float32)):
+        z = net.logits(x.permute(0, 3, 1, 2))[0]
+    out = policy.action_logprobs(z, move, mask=policy.legal_from_features(x), top=3)
+    hit = (out.top_action == move[:, None]).any(dim=1)
+    return torch.stack([torch.where(played, t.double(), 0.0).sum() for t in (out.entropy, out.logp, hit, played)])
 
 
 class History:
@@ -402,7 +406,7 @@ def train_nn(training_data, neural_network, **kwargs):
         else:
             acc = torch.zeros(3, dtype=torch.float64, device=dev)
         pen_eval = None if train else l2_penalty_value(net)
-        figures = torch.zeros(3, dtype=torch.float64, device=dev)
+        figures = torch.zeros(4, dtype=torch.float64, device=dev)
         rows_seen = 0
         for b in batches:
             sel = idx[b * BATCH_SIZE:(b + 1) * BATCH_SIZE]
@@ -439,10 +443,10 @@ def train_nn(training_data, neural_network, **kwargs):
                 with torch.no_grad():
                     loss, ce, mse = losses(net, x, pi, tv, amp, with_penalty=False, entropy_weight=entropy_weight)
                     if policy_metrics:
-                        figures += policy_figures(net, x, pi)
+                        figures += policy_figures(net, x, pi, amp)
                 acc += torch.stack([loss.detach() + pen_eval, ce.detach(), mse.detach()]).double() * float(sel.shape[0])
         if not train and policy_metrics:
-            entropy, logp, top3 = (figures / float(rows_seen)).tolist()
+            entropy, logp, top3, _ = (figures / figures[3]).tolist()        # (NaN where no row has visits)
             history.add(val_policy_entropy=entropy, val_move_logp=logp, val_move_top3=top3)
         tot, ce_s, mse_s = (acc / float(rows_seen)).tolist()
         return tot, ce_s, mse_s

@@ -547,3 +547,63 @@ def test_entropy_weight_and_policy_figures_of_training():
     assert abs(float(figures[0] - ref[1].sum())) <= 64 * bound(512) * 20
     hits = (ref[2] == pi.argmax(1)[:, None]).any(1).sum()
     assert float(figures[2]) == float(hits)
+
+
+def test_policy_figures_of_positions_without_visits():
+    """Games that run to their end leave terminal tuples: no visits, no legal move.  The figures are those of the other rows."""
+    from checkers_mcts_amd import engine as E, policy, train
+    from test_engine_gpu import mk, run_engine
+    eng, ev = run_engine(E, mk(6), [3, 4, 5], games_per_slot=2, terminate_cnt=400)
+    eng.run(ev)
+    data = train.TrainingData(tuples=eng.pack_tuples_device())
+    x, pi, tv = data.batch(torch.arange(len(data), device="cuda"))
+    eng.close()
+    played = pi.sum(1) > 0
+    assert 0 < int((~played).sum()) < 64 and not policy.legal_from_features(x)[~played].any()
+    net = train.create_nn(NUM_KERNELS=32, CONV_REG=1e-3, DENSE_REG=1e-3, POLICY_LOSS_WEIGHT=1.0, VALUE_LOSS_WEIGHT=1.0, SEED=2).cuda().eval()
+    sel = torch.cat([torch.nonzero(~played)[:, 0], torch.nonzero(played)[:200, 0]])
+    x, pi, tv, played = x[sel], pi[sel], tv[sel], played[sel]
+    with torch.no_grad():
+        z, _ = net.logits(x[played].permute(0, 3, 1, 2))
+    move = pi[played].argmax(1)
+    ref = reference(z, policy.legal_from_features(x[played]), move[:, None], 3, 1.0)
+    n = int(played.sum())
+    figures = train.policy_figures(net, x, pi).tolist()
+    assert figures[3] == n
+    # a library convolution over another batch may sum in another order: 1e-5 of a logit, as the network's own tests have it
+    assert abs(figures[0] - float(ref[1].sum())) <= n * (20 * bound(512) + 1e-4) and abs(figures[1] - float(ref[0].sum())) <= n * (2 * bound(512) + 1e-4)
+    assert abs(figures[2] - float((ref[2] == move[:, None]).any(1).sum())) <= 2          # two nearly equal candidates may change places
+    none = train.policy_figures(net, x[~played], pi[~played]).tolist()
+    assert none == [0.0, 0.0, 0.0, 0.0]
+    with torch.autocast("cuda", dtype=torch.bfloat16), torch.no_grad():
+        z16, _ = net.logits(x[played].permute(0, 3, 1, 2))
+    ref = reference(z16, policy.legal_from_features(x[played]), move[:, None], 3, 1.0)
+    half = train.policy_figures(net, x, pi, torch.bfloat16).tolist()                     # as the losses beside them are computed
+    # bfloat16 logits of size |z|: a last bit up or down is 2^-7 |z|, in the row's sum too
+    assert abs(half[1] - float(ref[0].sum())) <= n * (2 * bound(512) + 2 * 2.0 ** -7 * float(z16.abs().max()))
+
+
+def test_train_nn_policy_metrics_of_whole_games(tmp_path, monkeypatch):
+    import numpy as np
+    from checkers_mcts_amd import engine as E, train
+    from test_engine_gpu import mk, run_engine
+    monkeypatch.chdir(tmp_path)
+    eng, ev = run_engine(E, mk(6), [3, 4, 5], games_per_slot=2, terminate_cnt=400)
+    eng.run(ev)
+    tuples = eng.pack_tuples_device()
+    eng.close()
+    data = train.TrainingData(tuples=tuples)
+    _, pi, _ = data.batch(torch.arange(len(data), device="cuda"))
+    last = torch.nonzero(pi.sum(1) == 0)[:, 0]
+    assert len(last)
+    kw = dict(PATIENCE=5, MIN_DELTA=0, VAL_SPLIT=0.5, TRAINING_ITERATION=0, BATCH_SIZE=32, CLR_SS_COEFF=4, NN_BASE_LR=1e-4, NN_MAX_LR=1e-3, EPOCHS=2, NUM_KERNELS=32,
+              CONV_REG=1e-4, DENSE_REG=1e-4, POLICY_LOSS_WEIGHT=1.0, VALUE_LOSS_WEIGHT=1.0, SEED=1, TRAIN_BACKEND="torch", POLICY_METRICS=True)
+    # every second row of the job is one of a game's end
+    many = torch.cat([tuples[:200], tuples[last].repeat(200 // len(last) + 1, 1)])
+    history, _ = train.train_nn(many.contiguous(), train.create_nn(**kw), **kw)
+    h = history.history
+    assert all(np.isfinite(h[k]).all() for k in ("val_policy_entropy", "val_move_logp", "val_move_top3"))
+    assert max(h["val_move_logp"]) < 0 and min(h["val_policy_entropy"]) > 0 and 0 <= min(h["val_move_top3"]) <= 1
+    only = tuples[last].repeat(200 // len(last) + 1, 1).contiguous()                     # nothing to speak of
+    h = train.train_nn(only, train.create_nn(**kw), **kw)[0].history
+    assert all(np.isnan(h[k]).all() for k in ("val_policy_entropy", "val_move_logp", "val_move_top3"))
