@@ -21,6 +21,25 @@ _SHAPE, _DTYPE, _GRAD, _NBYTES = attrgetter("shape"), attrgetter("dtype"), attrg
 _STRIDE, _DEVICE, _POINTER = torch.Tensor.stride, torch.Tensor.get_device, torch.Tensor.data_ptr
 
 
+def _guards():
+    """torch's native comparison of many tensors' types, devices, sizes and strides with those of examples, if it sees all that matters
+    here: one call instead of six map()s over the parameters (a step of 170 tensors, wall time: 79 us, 97 us with the map()s)."""
+    try:
+        from torch._C._dynamo.guards import TensorGuards
+        x = torch.zeros((4, 4), dtype=torch.float16)
+        make = lambda *tensors: TensorGuards(*tensors, dynamic_dims_sizes=None, dynamic_dims_strides=None)
+        g, row = make(x, x), make(x[0])
+        others = (x.t(), x[:2], x.view(torch.bfloat16), x.view(torch.int16), x.to("meta"), x.reshape(2, 8), x[None], torch._neg_view(x), x.to_sparse(), None)
+        if g.check(x, torch.ones_like(x)) and row.check(x[1]) and not row.check(x[:, 0]) and not any(g.check(x, y) or g.check(y, x) for y in others):
+            return make
+    except Exception:                                                  # (not a public name: another torch may not have it, or in another form)
+        pass
+    return None
+
+
+_make_guards = _guards()
+
+
 class AdamWArgs(C.Structure):
     """ckr_adamw_args (include/ckr.h)."""
     _fields_ = [(n, C.c_void_p) for n in ("sizes", "offsets", "params", "grads", "master", "m", "v", "m_scale", "v_scale",
@@ -132,6 +151,7 @@ class AdamW:
         self._layouts = [_layout(p) for p in self._every]
         self._shape_of, self._stride_of, self._type_of, self._nbytes_of = ([f(p) for p in self._every] for f in (_SHAPE, _STRIDE, _DTYPE, _NBYTES))
         self._device_of = [dev.index] * first
+        self._guards = None                                            # of parameters and gradients that were found to be as above
         self._adopt()
         self._streams = {torch.cuda.current_stream(dev).cuda_stream}
         torch.cuda.current_stream(dev).synchronize()                   # a step on any stream finds the states in place
@@ -170,13 +190,17 @@ class AdamW:
             self._adopt()
             addresses = self._addresses
         gs = list(map(_GRAD, ps))
+        if self._guards is not None and self._guards.check(*ps, *gs):
+            return array("Q", addresses), array("Q", map(_POINTER, gs)), keep
+        if list(map(_STRIDE, ps)) != self._stride_of or list(map(_DTYPE, ps)) != self._type_of:      # the same memory, seen otherwise
+            self._adopt()
         try:
-            if list(map(_STRIDE, gs)) == self._stride_of and list(map(_NBYTES, gs)) == self._nbytes_of and list(map(_DEVICE, gs)) == self._device_of:
+            if list(map(_STRIDE, gs)) == self._stride_of and list(map(_DTYPE, gs)) == self._type_of and list(map(_NBYTES, gs)) == self._nbytes_of \
+                    and list(map(_DEVICE, gs)) == self._device_of:
+                self._guards = None if _make_guards is None else _make_guards(*ps, *gs)
                 return array("Q", addresses), array("Q", map(_POINTER, gs)), keep
         except (TypeError, AttributeError, RuntimeError):              # None, or sparse
             pass
-        if list(map(_STRIDE, ps)) != self._stride_of:                  # the same memory, seen otherwise
-            self._adopt()
         gs = [self._gradient(i, g, keep) for i, g in enumerate(gs)]
         return array("Q", addresses), array("Q", (0 if g is None else g.data_ptr() for g in gs)), keep
 

@@ -650,3 +650,60 @@ def test_train_nn_with_these_operators(optimizer, tmp_path, monkeypatch):
         got.append(net)
     with pytest.raises(ValueError, match="TRAIN_BACKEND"):
         train.train_nn(data, train.create_nn(**dict(kw, NUM_KERNELS=128)), **dict(kw, TRAIN_BACKEND="hip"))
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_a_parameter_seen_otherwise_beside_the_gradient_it_had_is_refused(native, monkeypatch):
+    from checkers_mcts_amd import optim
+    if not native:                                                    # as on a torch without the native comparison
+        monkeypatch.setattr(optim, "_make_guards", None)
+    p = torch.arange(64.0, device="cuda").reshape(8, 8).requires_grad_(True)
+    opt = optim.AdamW([p])
+    p.grad = torch.arange(64.0, device="cuda").reshape(8, 8) - 30
+    opt.step()
+    before = p.detach().clone()
+    p.data = p.data.t()
+    for again in (False, True):
+        if again:
+            (p * 2.0).sum().backward()                                # autograd adds to the gradient that is there, in its order
+        assert p.grad.stride() == (8, 1) and p.stride() == (1, 8)
+        with pytest.raises(ValueError):
+            opt.step()
+        assert torch.equal(p.detach().t(), before) and int(opt.steps[0]) == 1
+    p.data = p.data.t()                                               # as it was
+    opt.step()
+    assert int(opt.steps[0]) == 2
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("kept", [False, True])
+def test_a_parameter_of_another_type_at_the_same_address_is_refused(kept, native, monkeypatch):
+    from checkers_mcts_amd import optim
+    if not native:
+        monkeypatch.setattr(optim, "_make_guards", None)
+    p = torch.ones(64, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    opt = optim.AdamW([p])
+    p.grad = torch.ones_like(p)
+    opt.step()
+    p.data = p.data.view(torch.float16)
+    if not kept:
+        p.grad = torch.ones(64, device="cuda", dtype=torch.float16)
+    before = p.detach().clone()
+    with pytest.raises(ValueError):
+        opt.step()
+    assert torch.equal(p.detach(), before) and int(opt.steps[0]) == 1
+
+
+@pytest.mark.skipif(not hasattr(torch.Tensor, "grad_dtype"), reason="gradients have their parameters' type")
+def test_a_gradient_of_another_type_is_refused():
+    from checkers_mcts_amd import optim
+    p = torch.ones(64, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    opt = optim.AdamW([p])
+    p.grad = torch.ones_like(p)
+    opt.step()
+    p.grad = None
+    p.grad_dtype = torch.float16
+    p.grad = torch.ones(64, device="cuda", dtype=torch.float16)
+    with pytest.raises(ValueError):
+        opt.step()
+    assert int(opt.steps[0]) == 1
