@@ -19,6 +19,7 @@ DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # accessors for map(): a step looks at every parameter and gradient
 _SHAPE, _DTYPE, _GRAD, _NBYTES = attrgetter("shape"), attrgetter("dtype"), attrgetter("grad"), attrgetter("nbytes")
 _STRIDE, _DEVICE, _POINTER = torch.Tensor.stride, torch.Tensor.get_device, torch.Tensor.data_ptr
+_NEGATED = torch.Tensor.is_neg      # memory that holds the opposite sign: the gradient of an imaginary part, of one element, may come so
 
 
 def _guards():
@@ -110,6 +111,8 @@ class AdamW:
                 raise ValueError("parameters must be float32, bfloat16 or float16 tensors on one GPU")
             if not p.is_leaf:
                 raise ValueError("AdamW steps leaf tensors only")
+            if p.is_neg():
+                raise ValueError("a parameter is a view of the negative of its memory")
             if _layout(p) is None:
                 raise ValueError("a parameter of shape %s and strides %s does not fill its memory" % (list(p.shape), list(p.stride())))
         spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in every if p.numel())
@@ -196,7 +199,7 @@ class AdamW:
             self._adopt()
         try:
             if list(map(_STRIDE, gs)) == self._stride_of and list(map(_DTYPE, gs)) == self._type_of and list(map(_NBYTES, gs)) == self._nbytes_of \
-                    and list(map(_DEVICE, gs)) == self._device_of:
+                    and list(map(_DEVICE, gs)) == self._device_of and not any(map(_NEGATED, gs)):
                 self._guards = None if _make_guards is None else _make_guards(*ps, *gs)
                 return array("Q", addresses), array("Q", map(_POINTER, gs)), keep
         except (TypeError, AttributeError, RuntimeError):              # None, or sparse
@@ -219,7 +222,7 @@ class AdamW:
             raise ValueError("sparse gradients are not supported")
         if g.shape != self._shape_of[i] or g.dtype != self._type_of[i] or g.device != self.device:
             raise ValueError("a gradient must have its parameter's shape, type and device")
-        if _layout(g) != self._layouts[i]:
+        if _layout(g) != self._layouts[i] or g.is_neg():               # (a copy of a view of the negative holds its values)
             g = torch.empty_strided(g.shape, self._stride_of[i], dtype=g.dtype, device=g.device).copy_(g.detach())
             keep.append(g)
         return g

@@ -707,3 +707,22 @@ def test_a_gradient_of_another_type_is_refused():
     with pytest.raises(ValueError):
         opt.step()
     assert int(opt.steps[0]) == 1
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("shape", [(), (1,), (1, 1)], ids=str)
+def test_gradients_that_are_seen_negated(shape, native, monkeypatch):
+    """The gradient of an imaginary part may come as a view of its conjugate: the memory holds the opposite sign."""
+    from checkers_mcts_amd import optim
+    if not native:
+        monkeypatch.setattr(optim, "_make_guards", None)
+    w, one = torch.zeros(shape, device="cuda", requires_grad=True), torch.ones(shape, device="cuda")
+    opt = optim.AdamW([w], lr=0.5, weight_decay=0.0, max_norm=10.0)
+    (torch.complex(one, w).conj() * torch.complex(one, 3 * one)).imag.sum().backward()   # (1 - i w) (1 + 3 i): 3 - w
+    assert w.grad.is_neg() and float(w.grad) == -1
+    opt.step()
+    assert abs(float(w.detach()) - 0.5) <= 0.5 * (16 * U + 1e-8)               # 12 u of the update, 2 of w, and eps beside 1
+    p = torch.complex(one, one).conj().imag.detach().requires_grad_(True)
+    assert p.is_neg() and p.is_leaf
+    with pytest.raises(ValueError, match="negative"):
+        optim.AdamW([p])
