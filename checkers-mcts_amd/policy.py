@@ -79,8 +79,9 @@ def _forward(x, actions, mask, mask_kind, top, inv_temperature, want_stats):
 
 
 def _f32(g):
-    """An output's gradient as the kernel reads it (sums and means hand expanded ones down)."""
-    return g if g is None or (g.dtype is torch.float32 and g.is_contiguous()) else g.float().contiguous()
+    """An output's gradient as the kernel reads it (sums and means hand expanded ones down, an imaginary part's may be a view of the
+    negative of its memory)."""
+    return g if g is None or (g.dtype is torch.float32 and g.is_contiguous() and not g.is_neg()) else g.float().contiguous().resolve_neg()
 
 
 class _Logprobs(torch.autograd.Function):

@@ -607,3 +607,19 @@ def test_train_nn_policy_metrics_of_whole_games(tmp_path, monkeypatch):
     only = tuples[last].repeat(200 // len(last) + 1, 1).contiguous()                     # nothing to speak of
     h = train.train_nn(only, train.create_nn(**kw), **kw)[0].history
     assert all(np.isnan(h[k]).all() for k in ("val_policy_entropy", "val_move_logp", "val_move_top3"))
+
+
+def test_gradients_that_are_seen_negated():
+    """The gradient of an imaginary part may come as a view of its conjugate: the memory holds the opposite sign."""
+    from checkers_mcts_amd import policy
+    x, a, _ = make(1, 700, torch.float32, 5)
+    a = a.clamp(min=0)[:, 0]
+    for name in ("logp", "entropy"):
+        leaf = x.clone().requires_grad_(True)
+        out = getattr(policy.action_logprobs(leaf, a), name)
+        one = torch.ones_like(out)
+        want, = torch.autograd.grad(out, leaf, -one, retain_graph=True)
+        seen = []
+        out.register_hook(lambda g: seen.append(g.is_neg()))
+        got, = torch.autograd.grad((torch.complex(one, out).conj() * torch.complex(one, 3 * one)).imag.sum(), leaf)      # 3 - out
+        assert seen == [True] and torch.equal(got, want)
