@@ -345,15 +345,24 @@ class AdamW:
 
     @torch.no_grad()
     def load_state_dict(self, state):
+        """A learning rate on the device keeps its scalar, which takes the saved value: captured steps go on reading it."""
         if state["state_bits"] != self.state_bits or state["sizes"] != [p.numel() for p in self.params] or len(state["param_groups"]) != len(self.param_groups) \
                 or (state["master"] is None) != (self.master is None) or state["steps"].numel() != self.steps.numel():
             raise ValueError("the state belongs to other parameters, groups or state_bits")
+        groups = []
         for g, new in zip(self.param_groups, state["param_groups"]):
+            new = dict(new)
+            if isinstance(new.get("lr"), torch.Tensor):                # of another device, or another optimiser's own
+                new["lr"] = new["lr"].to(self.device, copy=True)
             self._check_group(dict(g, **new))
+            groups.append(new)
         for mine, other in ((self.exp_avg, state["exp_avg"]), (self.exp_avg_sq, state["exp_avg_sq"]), (self.scales, state["scales"]),
                             (self.master, state["master"]), (self.steps, state["steps"])):
             if mine is not None:
                 mine.copy_(other)
         self.seed = state["seed"]
-        for g, new in zip(self.param_groups, state["param_groups"]):
+        for g, new in zip(self.param_groups, groups):
+            if isinstance(g["lr"], torch.Tensor) and "lr" in new:
+                value = new.pop("lr")
+                g["lr"].copy_(value.reshape(g["lr"].shape)) if isinstance(value, torch.Tensor) else g["lr"].fill_(float(value))
             g.update(new)

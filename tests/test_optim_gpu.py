@@ -726,3 +726,59 @@ def test_gradients_that_are_seen_negated(shape, native, monkeypatch):
     assert p.is_neg() and p.is_leaf
     with pytest.raises(ValueError, match="negative"):
         optim.AdamW([p])
+
+
+def test_a_checkpoint_of_a_learning_rate_on_the_device(tmp_path):
+    """Loading keeps the scalar that the caller fills and captured steps read; nothing is shared with the optimiser it came from."""
+    from checkers_mcts_amd import optim
+    scalar = lambda v: torch.tensor(v, device="cuda")
+
+    def build(lr):
+        ps = [p.requires_grad_(True) for p in make((300, 70), torch.float32, 3)]
+        for p, g in zip(ps, make((300, 70), torch.float32, 4)):
+            p.grad = g
+        return ps, optim.AdamW(ps, lr=lr, weight_decay=0.0)
+    ps, opt = build(scalar(1e-2))
+    opt.step()
+    qs, other = build(mine := scalar(5.0))
+    other.load_state_dict(opt.state_dict())
+    assert other.param_groups[0]["lr"] is mine and mine.data_ptr() != opt.param_groups[0]["lr"].data_ptr() and float(mine) == float(opt.param_groups[0]["lr"])
+    mine.fill_(0.25)
+    assert float(opt.param_groups[0]["lr"]) == float(scalar(1e-2))
+    # a captured step goes on reading it
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        other.step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        other.step()
+    other.load_state_dict(opt.state_dict())                           # lr 1e-2 again
+    with torch.no_grad():
+        for p, q in zip(ps, qs):
+            q.copy_(p)
+    for _ in range(3):
+        graph.replay()
+        opt.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+    # from a file, mapped to the host; a number where the saved one is on the device, and the other way round
+    torch.save(opt.state_dict(), tmp_path / "o.pt")
+    saved = torch.load(tmp_path / "o.pt", map_location="cpu", weights_only=True)
+    for lr in (scalar(3.0), 3.0):
+        rs, third = build(lr)
+        third.load_state_dict(saved)
+        now = third.param_groups[0]["lr"]
+        assert now.is_cuda and now.dtype == torch.float32 and float(now) == float(scalar(1e-2)) and torch.equal(third.exp_avg, opt.exp_avg)
+        third.step()
+    _, fourth = build(0.125)
+    rs, third = build(mine := scalar(3.0))
+    third.load_state_dict(fourth.state_dict())
+    assert third.param_groups[0]["lr"] is mine and float(mine) == 0.125
+    bad = opt.state_dict()
+    bad["param_groups"][0]["lr"] = torch.ones(2)
+    before = [t.clone() for t in (third.exp_avg, third.steps)]
+    with pytest.raises(ValueError):
+        third.load_state_dict(bad)
+    assert torch.equal(before[0], third.exp_avg) and torch.equal(before[1], third.steps) and float(mine) == 0.125
