@@ -154,6 +154,8 @@ class AdamW:
         self._layouts = [_layout(p) for p in self._every]
         self._shape_of, self._stride_of, self._type_of, self._nbytes_of = ([f(p) for p in self._every] for f in (_SHAPE, _STRIDE, _DTYPE, _NBYTES))
         self._device_of = [dev.index] * first
+        # what the order of the states follows from: each group's parameters, their types and, where they are not row by row, how they lie
+        self._arrangement = [[[str(p.dtype)] + ([] if p.is_contiguous() else [list(n) for n in _layout(p)]) for p in g["params"]] for g in groups]
         self._guards = None                                            # of parameters and gradients that were found to be as above
         self._adopt()
         self._streams = {torch.cuda.current_stream(dev).cuda_stream}
@@ -339,7 +341,7 @@ class AdamW:
     def state_dict(self):
         """States (the buffers themselves) and hyperparameters; load_state_dict() of an optimiser over the same parameters takes it.  The
         parameters are not among them, the master copies of 16-bit ones are."""
-        return {"state_bits": self.state_bits, "seed": self.seed, "exp_avg": self.exp_avg, "exp_avg_sq": self.exp_avg_sq, "scales": self.scales,
+        return {"layout": self._arrangement, "state_bits": self.state_bits, "seed": self.seed, "exp_avg": self.exp_avg, "exp_avg_sq": self.exp_avg_sq, "scales": self.scales,
                 "master": self.master, "steps": self.steps, "sizes": [p.numel() for p in self.params],
                 "param_groups": [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups]}
 
@@ -349,6 +351,9 @@ class AdamW:
         if state["state_bits"] != self.state_bits or state["sizes"] != [p.numel() for p in self.params] or len(state["param_groups"]) != len(self.param_groups) \
                 or (state["master"] is None) != (self.master is None) or state["steps"].numel() != self.steps.numel():
             raise ValueError("the state belongs to other parameters, groups or state_bits")
+        if state.get("layout", self._arrangement) != self._arrangement:     # (states saved before it was among them: as they are)
+            raise ValueError("the state belongs to parameters of other types, orders in memory or groups; moments() with split(), and load_moments(), "
+                             "carry moments over")
         groups = []
         for g, new in zip(self.param_groups, state["param_groups"]):
             new = dict(new)

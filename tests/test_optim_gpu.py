@@ -782,3 +782,41 @@ def test_a_checkpoint_of_a_learning_rate_on_the_device(tmp_path):
     with pytest.raises(ValueError):
         third.load_state_dict(bad)
     assert torch.equal(before[0], third.exp_avg) and torch.equal(before[1], third.steps) and float(mine) == 0.125
+
+
+def test_a_checkpoint_of_parameters_that_lie_otherwise_is_refused():
+    """Moments are kept in the order of the parameters' memory, step counts in the order of groups and types."""
+    from checkers_mcts_amd import optim
+    param = lambda t: t.cuda().requires_grad_(True)
+    conv = torch.arange(2.0 * 3 * 4 * 4).reshape(2, 3, 4, 4)
+
+    def saved(params):
+        opt = optim.AdamW(params)
+        for p in opt.params:
+            p.grad = torch.ones_like(p)
+        opt.step()
+        return opt.state_dict()
+    there = conv.contiguous(memory_format=torch.channels_last)
+    for one, other in ((conv, there), (there, conv), (there, conv.permute(1, 0, 2, 3).contiguous().permute(1, 0, 2, 3))):
+        with pytest.raises(ValueError):
+            optim.AdamW([param(one)]).load_state_dict(saved([param(other)]))
+    for one, other in ((conv, conv.reshape(-1)), (there, there.clone()), (torch.ones(5, 6, 1, 1), torch.ones(5, 6, 1, 1).contiguous(memory_format=torch.channels_last))):
+        optim.AdamW([param(one)]).load_state_dict(saved([param(other)]))
+    # the same sizes, types in another order
+    a, b = torch.ones(100), torch.ones(100).bfloat16()
+    here = saved([param(a), param(b)])
+    with pytest.raises(ValueError):
+        optim.AdamW([param(b), param(a)]).load_state_dict(here)
+    with pytest.raises(ValueError):
+        optim.AdamW([param(a), param(torch.ones(100).half())]).load_state_dict(here)
+    # the same tensors, divided into groups otherwise
+    three = lambda: [param(torch.ones(100)) for _ in range(3)]
+    groups = lambda ps, k: [{"params": ps[:k]}, {"params": ps[k:]}]
+    here = saved(groups(three(), 1))
+    with pytest.raises(ValueError):
+        optim.AdamW(groups(three(), 2)).load_state_dict(here)
+    other = optim.AdamW(groups(three(), 1))
+    other.load_state_dict(here)
+    assert other.steps.tolist() == [1, 1, 1]
+    old = {k: v for k, v in here.items() if k != "layout"}            # saved before the layout was part of it
+    other.load_state_dict(old)
