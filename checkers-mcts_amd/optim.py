@@ -18,6 +18,7 @@ TICKET_WORDS = 1056                 # CKR_TICKET_WORDS
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # accessors for map(): a step looks at every parameter and gradient
 _SHAPE, _DTYPE, _GRAD, _NBYTES = attrgetter("shape"), attrgetter("dtype"), attrgetter("grad"), attrgetter("nbytes")
+_VERSION = attrgetter("_version")
 _STRIDE, _DEVICE, _POINTER = torch.Tensor.stride, torch.Tensor.get_device, torch.Tensor.data_ptr
 _NEGATED = torch.Tensor.is_neg      # memory that holds the opposite sign: the gradient of an imaginary part, of one element, may come so
 
@@ -79,8 +80,8 @@ class AdamW:
 
     params        tensors, or groups {"params": [...], "lr": ..., "betas": ..., "eps": ..., "weight_decay": ...}, of float32, bfloat16
                   or float16 on one GPU, dense in memory (any order of dimensions).  16-bit parameters get a float32 master copy, which is
-                  what the optimiser updates; the parameter is its rounding.  Their memory may be replaced (p.data = ...) by some of the same
-                  shape, strides and type.
+                  what the optimiser updates; the parameter is its rounding, and where something else has changed it, the copy follows
+                  (reset_master()).  Their memory may be replaced (p.data = ...) by some of the same shape, strides and type.
     lr            a number, or a float32 device scalar (read by the kernel: a captured step follows its changes).
     state_bits    32, or 8: a byte for each moment and a scale byte for each 128 elements, rounded stochastically (seed).
     max_norm      clip the gradients by their global norm (over all groups): g * min(1, max_norm / (norm + 1e-6)); the norm of the last
@@ -139,7 +140,10 @@ class AdamW:
         z = lambda n, dtype: torch.zeros((n,), dtype=dtype, device=dev)
         self.exp_avg, self.exp_avg_sq = z(total, state), z(total, state)
         self.scales = (torch.ones((2, max(1, total // BLOCK)), dtype=torch.uint8, device=dev)) if self.state_bits == 8 else None
-        self.master = None
+        self._every = [p for b in self._batches for p in b.params]     # in the order of the batches
+        self._half = [i for i, p in enumerate(self._every) if p.dtype != torch.float32]
+        self._half_params = [self._every[i] for i in self._half]
+        self.master, self._versions = None, []
         if any(p.dtype != torch.float32 for p in every):
             self.master = z(total, torch.float32)
             self.reset_master()
@@ -148,12 +152,11 @@ class AdamW:
         # partial sums of the norm: one launch for each run of up to TENSORS tensors of one type
         launches = sum((b.n + TENSORS - 1) // TENSORS for b in self._batches)
         self._parts, self._norm = (z(max(1, launches) * BLOCKS, torch.float64), z(2, torch.float64)) if self._max_norm is not None else (None, None)
-        self._every = [p for b in self._batches for p in b.params]     # in the order of the batches
         self._sizes_all = (C.c_int64 * first)(*[p.numel() for p in self._every])
         self._dtypes_all = (C.c_int32 * first)(*[DTYPES[p.dtype] for p in self._every])
         self._layouts = [_layout(p) for p in self._every]
         self._shape_of, self._stride_of, self._type_of, self._nbytes_of = ([f(p) for p in self._every] for f in (_SHAPE, _STRIDE, _DTYPE, _NBYTES))
-        self._device_of = [dev.index] * first
+        self._device_of, self._offset_of = [dev.index] * first, [where[id(p)] for p in self._every]
         # what the order of the states follows from: each group's parameters, their types and, where they are not row by row, how they lie
         self._arrangement = [[[str(p.dtype)] + ([] if p.is_contiguous() else [list(n) for n in _layout(p)]) for p in g["params"]] for g in groups]
         self._guards = None                                            # of parameters and gradients that were found to be as above
@@ -192,8 +195,13 @@ class AdamW:
         ps, keep = self._every, []
         addresses = list(map(_POINTER, ps))
         if addresses != self._addresses:                               # (_aliases keep the memory: at the same address it is the same)
+            moved = [i for i in self._half if addresses[i] != self._addresses[i]]
             self._adopt()
+            self._follow(moved)
             addresses = self._addresses
+        if self._half and (versions := list(map(_VERSION, self._half_params))) != self._versions:
+            self._follow([i for i, now, then in zip(self._half, versions, self._versions) if now != then])
+            self._versions = versions
         gs = list(map(_GRAD, ps))
         if self._guards is not None and self._guards.check(*ps, *gs):
             return array("Q", addresses), array("Q", map(_POINTER, gs)), keep
@@ -216,6 +224,17 @@ class AdamW:
                 raise ValueError("a parameter's shape, strides, type or device changed after the optimiser was made")
         self._aliases = [p.detach() for p in self._every]
         self._addresses = list(map(_POINTER, self._every))
+
+    @torch.no_grad()
+    def _follow(self, which):
+        """Something else than a step has changed these 16-bit parameters: where one is no longer the rounding of its master copy, the copy
+        takes its value."""
+        for i in which:
+            p = self._every[i]
+            if p.shape != self._shape_of[i] or p.stride() != self._stride_of[i] or p.dtype != self._type_of[i]:
+                raise ValueError("a parameter's shape, strides, type or device changed after the optimiser was made")
+            master = self._flat_view(self.master, p, self._offset_of[i])
+            master.copy_(torch.where(master.to(p.dtype) == p.detach(), master, p.detach().float()))
 
     def _gradient(self, i, g, keep):
         if g is None:
@@ -264,6 +283,8 @@ class AdamW:
         stepped = self._every if 0 not in gs else [p for p, g in zip(self._every, gs) if g]
         if stepped:
             torch.autograd.graph.increment_version(stepped)            # a backward pass over what it saved before the step is refused
+        if self._half:
+            self._versions = list(map(_VERSION, self._half_params))    # (views of one buffer share a counter: not simply one more)
 
     @property
     def max_norm(self):
@@ -285,11 +306,13 @@ class AdamW:
 
     @torch.no_grad()
     def reset_master(self):
-        """Takes the master copies from the 16-bit parameters: after something else than step() has changed them (load_state_dict() of the
-        module, say), which the next step would otherwise undo."""
+        """Takes the master copies from the 16-bit parameters.  step() sees by itself what has changed them in place (load_state_dict() of the
+        module, say) or replaced their memory.  What torch's version counters do not show (p.data.copy_(), another replayed graph) it
+        would undo, and the replay of a captured step undoes any change: call this first."""
         for p, o in zip(self.params, self.offsets):
             if p.dtype != torch.float32:
                 self._flat_view(self.master, p, o).copy_(p.detach())
+        self._versions = list(map(_VERSION, self._half_params))
 
     # ---- states ---------------------------------------------------------------------------------------------
     def moments(self):
@@ -365,6 +388,7 @@ class AdamW:
                             (self.master, state["master"]), (self.steps, state["steps"])):
             if mine is not None:
                 mine.copy_(other)
+        self._versions = list(map(_VERSION, self._half_params))        # the masters are the state's
         self.seed = state["seed"]
         for g, new in zip(self.param_groups, groups):
             if isinstance(g["lr"], torch.Tensor) and "lr" in new:

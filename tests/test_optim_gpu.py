@@ -820,3 +820,74 @@ def test_a_checkpoint_of_parameters_that_lie_otherwise_is_refused():
     assert other.steps.tolist() == [1, 1, 1]
     old = {k: v for k, v in here.items() if k != "layout"}            # saved before the layout was part of it
     other.load_state_dict(old)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("bits", [32, 8])
+def test_what_else_changes_a_16_bit_parameter_is_not_undone(dtype, bits):
+    """A module's weights loaded after the optimiser was made, or other memory with other values: the master copies follow where the
+    parameter is no longer their rounding, and stay where it is."""
+    from checkers_mcts_amd import optim
+    a, b = (p.requires_grad_(True) for p in make((1000, 64), dtype, 3, 1.0))
+    opt = optim.AdamW([a, b], lr=1e-4, weight_decay=0.0, state_bits=bits)
+    for p, g in zip((a, b), make((1000, 64), dtype, 4)):
+        p.grad = g
+    opt.step()
+    masters = [m.clone() for m in opt.split(opt.master)]
+    assert not torch.equal(masters[0], a.detach().float())
+    still = torch.zeros(1000, dtype=torch.bool, device="cuda")
+    still[::2] = True
+    new = torch.where(still, a.detach(), a.detach() + 1)
+    assert bool((new != a)[~still].all())
+    with torch.no_grad():
+        a.copy_(new)
+    for p in (a, b):
+        p.grad = torch.zeros_like(p)
+    for g in opt.param_groups:
+        g["lr"] = 0.0
+    opt.step()                                                        # of size zero
+    assert torch.equal(a.detach(), new)
+    now = opt.split(opt.master)
+    assert torch.equal(now[0][still], masters[0][still]) and torch.equal(now[0][~still], new.float()[~still]) and torch.equal(now[1], masters[1])
+    # other memory
+    more = new + 2
+    a.data = more.clone()
+    opt.step()
+    assert torch.equal(a.detach(), more) and torch.equal(opt.split(opt.master)[0], more.float()) and torch.equal(opt.split(opt.master)[1], masters[1])
+    # without a gradient it is nobody's turn
+    a.grad = None
+    with torch.no_grad():
+        a.fill_(7.0)
+    opt.step()
+    assert (a == 7).all()
+    # the state of a checkpoint is the state: its masters are not taken from parameters that were changed before
+    state = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in opt.state_dict().items()}
+    state["master"].fill_(3.0)
+    with torch.no_grad():
+        b.fill_(9.0)
+    opt.load_state_dict(state)
+    b.grad = torch.zeros_like(b)
+    opt.step()
+    assert (b == 3).all()
+
+
+def test_steps_of_16_bit_parameters_in_one_buffer_are_not_taken_for_changes(monkeypatch):
+    """Views of one buffer share a version counter."""
+    from checkers_mcts_amd import optim
+    flat = torch.ones(300, device="cuda", dtype=torch.bfloat16)
+    ps = [flat[i:i + 100].detach().requires_grad_(True) for i in (0, 100, 200)]
+    opt = optim.AdamW(ps, lr=1e-4)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    followed = []
+    whole = opt._follow
+    monkeypatch.setattr(opt, "_follow", lambda which: (followed.append(list(which)), whole(which)))
+    for s in range(4):
+        if s == 2:
+            ps[1].grad = None
+        opt.step()
+    assert followed == [] and (opt.split(opt.master)[0] < 1).all()
+    flat[250:].fill_(5.0)
+    ps[2].grad = torch.zeros_like(ps[2])
+    opt.step()
+    assert followed == [[0, 1, 2]] and (ps[2].detach()[50:] > 4).all() and (ps[2].detach()[:50] < 1.01).all()
