@@ -9,6 +9,7 @@ import functools
 from collections import namedtuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, rules
 
@@ -113,6 +114,19 @@ class _Logprobs(torch.autograd.Function):
         return (grad,) + (None,) * 5
 
 
+def _check_derivatives(logits):
+    """Refuses what would get outputs without knowing how they came about: kernels leave no trace in torch's records, and autograd takes part
+    in reverse mode alone."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(logits).tangent is not None:
+        raise ValueError("action_logprobs has no forward-mode derivative")
+    recorded = torch.jit.is_tracing()
+    if not recorded and torch._C._len_torch_dispatch_stack():
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+        recorded = get_proxy_mode() is not None
+    if recorded:
+        raise ValueError("action_logprobs cannot be recorded by torch.jit.trace or make_fx")
+
+
 def _check_mask(mask, lead, v, device):
     """-> (mask with one row or a row per row of logits, kind)."""
     if not isinstance(mask, torch.Tensor) or mask.device != device:
@@ -155,10 +169,11 @@ def action_logprobs(logits, actions=None, mask=None, top=0, temperature=1.0):
     -inf.  A row without an allowed action: log p -inf, entropy 0, gradient 0.  Where there are fewer than `top` alternatives: action
     -1, log p -inf.  NaN or +inf among the allowed logits make the row's numbers NaN and its alternatives -1.
 
-    Differentiable (once) in logits through logp and entropy; the alternatives are not.  A masked given action of a row with others keeps
+    Differentiable (once, in reverse mode) in logits through logp and entropy; the alternatives are not.  A masked given action of a row with others keeps
     its part in the gradient, - g p_j, as the formula has it."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dtype not in DTYPES or logits.dim() < 1:
         raise ValueError("logits must be a cuda float32, bfloat16 or float16 tensor [..., V]")
+    _check_derivatives(logits)
     lead, v = logits.shape[:-1], logits.shape[-1]
     if v < 1 or v > 1 << 30:
         raise ValueError("logits must have 1 to 2^30 actions a row, got %d" % v)

@@ -623,3 +623,30 @@ def test_gradients_that_are_seen_negated():
         out.register_hook(lambda g: seen.append(g.is_neg()))
         got, = torch.autograd.grad((torch.complex(one, out).conj() * torch.complex(one, 3 * one)).imag.sum(), leaf)      # 3 - out
         assert seen == [True] and torch.equal(got, want)
+
+
+def test_derivatives_that_are_not_there_are_refused():
+    """Forward-mode derivatives and recorded programs: neither would see what the kernels do."""
+    import torch.autograd.forward_ad as forward_ad
+    from checkers_mcts_amd import policy
+    x, a, _ = make(4, 20, torch.float32, 1)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for leaf in (dual, dual.reshape(2, 2, 20)):
+            with pytest.raises((ValueError, NotImplementedError)):
+                policy.action_logprobs(leaf)
+        with torch.no_grad(), pytest.raises((ValueError, NotImplementedError)):
+            policy.action_logprobs(dual, a)
+        inside = policy.action_logprobs(x, a)                          # without a tangent: as ever
+    assert all(torch.equal(p, q) for p, q in zip(inside[:2], policy.action_logprobs(x, a)[:2]))
+    entropy = lambda t: policy.action_logprobs(t).entropy
+    with pytest.raises((ValueError, RuntimeError)):
+        torch.func.jvp(entropy, (x,), (torch.ones_like(x),))
+    with pytest.raises((ValueError, RuntimeError)):
+        torch.func.vmap(entropy)(x[None])
+    with pytest.raises(ValueError, match="record"):
+        torch.jit.trace(entropy, (x,), check_trace=False)
+    from torch.fx.experimental.proxy_tensor import make_fx
+    with pytest.raises(ValueError, match="record"):
+        make_fx(entropy)(x)
+    assert torch.equal(entropy(x), policy.action_logprobs(x, a).entropy)
