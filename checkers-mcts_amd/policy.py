@@ -102,8 +102,10 @@ class _Logprobs(torch.autograd.Function):
             return (None,) * 6
         x, actions, mask, stats = ctx.saved_tensors
         grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        g_logp, g_entropy, a = _f32(g_logp), _f32(g_entropy), ctx.args
-        # the forward's arguments, with the tensors as they come back (hooks may have moved them)
+        g_logp, g_entropy = _f32(g_logp), _f32(g_entropy)
+        # the forward's arguments, with the tensors as they come back (hooks may have moved them); a copy, as passes over one graph may run at
+        # the same time
+        a = LogprobsArgs.from_buffer_copy(ctx.args)
         a.logits, a.stats, a.grad, a.grad_stride, a.top = x.data_ptr(), stats.data_ptr(), grad.data_ptr(), x.shape[1], 0
         a.row_stride = x.stride(0) if x.shape[0] > 1 else x.shape[1]
         a.g_logp, a.g_entropy, a.actions, a.mask, a.scratch = _ptr(g_logp), _ptr(g_entropy), _ptr(actions), _ptr(mask), None

@@ -120,3 +120,40 @@ def test_train_nn_refuses_what_cannot_run_together():
                        (dict(MAX_GRAD_NORM=1.0), "MAX_GRAD_NORM"), (dict(WEIGHT_DECAY=0.1), "WEIGHT_DECAY")):
         with pytest.raises(ValueError, match=word):
             train.train_nn(data, train.create_nn(**kw), **dict(kw, **more))
+
+
+def stubbed(monkeypatch, calls):
+    """policy's autograd function on host tensors: `calls` gets a copy of every structure that would have been launched."""
+    from checkers_mcts_amd import policy
+    monkeypatch.setattr(policy, "_call", lambda fn, a, device: calls(policy.LogprobsArgs.from_buffer_copy(a)))
+    return lambda x, a, mask=None, top=0: policy._Logprobs.apply(x, a, mask, policy.MASK_NONE if mask is None else policy.MASK_BYTES, top, 1.0)
+
+
+def test_two_backward_passes_of_one_graph_at_the_same_time(lib, monkeypatch):
+    """Without autograd's own threads each caller runs the function itself: what one fills in is not another's."""
+    import threading
+    inside, seen = threading.Barrier(2, timeout=20), []
+
+    def call(a):
+        if a.grad:
+            seen.append((a.grad, a.g_logp))
+    from checkers_mcts_amd import policy
+    x, a = torch.zeros(3, 7, requires_grad=True), torch.zeros((3, 2), dtype=torch.int64)
+    apply = stubbed(monkeypatch, lambda a: None)
+    logp, entropy, _, _ = apply(x, a)
+    monkeypatch.setattr(policy, "_call", lambda fn, a, device: (inside.wait(), call(a), inside.wait()))       # both have filled theirs in before either is looked at
+    gs, got, failed = [torch.full((3, 2), float(i)) for i in range(2)], [None, None], []
+
+    def run(i):
+        try:
+            with torch.autograd.set_multithreading_enabled(False):
+                got[i], = torch.autograd.grad(logp, x, gs[i], retain_graph=True)
+        except Exception as e:
+            failed.append(e)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not failed and len(seen) == 2
+    assert {g for g, _ in seen} == {g.data_ptr() for g in got} and {g for _, g in seen} == {g.data_ptr() for g in gs}
