@@ -85,11 +85,23 @@ def _f32(g):
     return g if g is None or (g.dtype is torch.float32 and g.is_contiguous() and not g.is_neg()) else g.float().contiguous().resolve_neg()
 
 
+def _kind(t):
+    return None if t is None else (t.dtype, t.shape, t.device)
+
+
+def _came_back(t, kind):
+    """A saved tensor as the kernel reads it: hooks may hand another one back."""
+    if _kind(t) != kind:
+        raise RuntimeError("action_logprobs: a saved tensor came back with another type, shape or device")
+    return t if t is None or t.dim() < 2 or t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
 class _Logprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, actions, mask, mask_kind, top, inv_temperature):
         logp, entropy, top_action, top_logp, stats, ctx.args = _forward(x, actions, mask, mask_kind, top, inv_temperature, True)
         ctx.save_for_backward(x, actions, mask, stats)
+        ctx.kinds = [_kind(t) for t in (x, actions, mask, stats)]
         ctx.set_materialize_grads(False)
         if top:
             ctx.mark_non_differentiable(top_action, top_logp)
@@ -100,7 +112,8 @@ class _Logprobs(torch.autograd.Function):
     def backward(ctx, g_logp, g_entropy, _action, _top):
         if g_logp is None and g_entropy is None:
             return (None,) * 6
-        x, actions, mask, stats = ctx.saved_tensors
+        x, actions, mask, stats = map(_came_back, ctx.saved_tensors, ctx.kinds)
+        actions, stats = actions if actions is None else actions.contiguous(), stats.contiguous()
         grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         g_logp, g_entropy = _f32(g_logp), _f32(g_entropy)
         # the forward's arguments, with the tensors as they come back (hooks may have moved them); a copy, as passes over one graph may run at

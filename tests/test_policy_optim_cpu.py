@@ -157,3 +157,37 @@ def test_two_backward_passes_of_one_graph_at_the_same_time(lib, monkeypatch):
         t.join(60)
     assert not failed and len(seen) == 2
     assert {g for g, _ in seen} == {g.data_ptr() for g in got} and {g for _, g in seen} == {g.data_ptr() for g in gs}
+
+
+@pytest.mark.parametrize("which", ["logits", "actions", "mask", "stats"])
+@pytest.mark.parametrize("change", ["type", "shape", "device"])
+def test_saved_tensors_that_come_back_as_others_are_refused(lib, monkeypatch, which, change):
+    seen = []
+    apply = stubbed(monkeypatch, seen.append)
+    x, a, mask = torch.zeros(3, 7, requires_grad=True), torch.zeros((3, 2), dtype=torch.int64), torch.ones(3, 7, dtype=torch.bool)
+    is_it = {"logits": lambda t: t.shape == (3, 7) and t.dtype == torch.float32, "actions": lambda t: t.dtype == torch.int64, "mask": lambda t: t.dtype == torch.bool,
+             "stats": lambda t: t.shape == (3, 4)}[which]
+    other = {"type": lambda t: t.to(torch.float64 if t.is_floating_point() else torch.int16), "shape": lambda t: t[:2], "device": lambda t: t.to("meta")}[change]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: other(t) if is_it(t) else t):
+        logp, entropy, _, _ = apply(x, a, mask)
+    forward = len(seen)
+    with pytest.raises(RuntimeError, match="saved"):
+        torch.autograd.grad((logp.sum() + entropy.sum()), x)
+    assert len(seen) == forward                                        # nothing was launched
+
+
+def test_saved_tensors_that_come_back_in_another_order_are_copied(lib, monkeypatch):
+    seen = []
+    apply = stubbed(monkeypatch, seen.append)
+    x, a, mask = torch.zeros(3, 7, requires_grad=True), torch.zeros((3, 2), dtype=torch.int64), torch.ones(3, 7, dtype=torch.bool)
+    keep = []
+
+    def turned(t):
+        keep.append(t.t().contiguous().t() if t.dim() == 2 else t)
+        return keep[-1]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, turned):
+        logp, entropy, _, _ = apply(x, a, mask)
+    torch.autograd.grad((logp.sum() + entropy.sum()), x)
+    addresses = {t.data_ptr() for t in keep}
+    b = seen[-1]
+    assert len(keep) == 4 and not addresses & {b.logits, b.actions, b.mask, b.stats} and (b.row_stride, b.mask_stride) == (7, 7)
