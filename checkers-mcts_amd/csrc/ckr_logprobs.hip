@@ -306,6 +306,9 @@ __device__ __forceinline__ void join_lanes(Sums& s, float c) {
     s.S = wave_sum_f32(s.S); s.D = wave_sum_f32(s.D);
 }
 
+// (x - max) it from halves: x - max itself may not fit (lowest against largest values) where the product does
+__device__ __forceinline__ float scaled(float x, float m, float it) { return (0.5f * x - 0.5f * m) * (2.0f * it); }
+
 template <typename T, int MASK, bool TOP>
 __device__ __forceinline__ void write_row(const Args& A, long long row, const Sums& s, const TopList& list) {
     const int lane = lane_id();
@@ -322,12 +325,12 @@ __device__ __forceinline__ void write_row(const Args& A, long long row, const Su
         float lp;
         if (a < 0) lp = 0.0f;
         else if (a >= A.v || bad) lp = __builtin_nanf("");
-        else lp = !empty && is_allowed<MASK>(A, row, (int)a) ? ((float)x[a] - s.m) * it - lnS : -__builtin_huge_valf();
+        else lp = !empty && is_allowed<MASK>(A, row, (int)a) ? scaled((float)x[a], s.m, it) - lnS : -__builtin_huge_valf();
         A.logp[row * A.n_given + lane] = lp;
     }
     if (TOP && lane < A.top) {
         A.top_action[row * A.top + lane] = bad ? -1 : list.i;
-        A.top_logp[row * A.top + lane] = bad ? __builtin_nanf("") : list.i < 0 ? -__builtin_huge_valf() : (list.v - s.m) * it - lnS;
+        A.top_logp[row * A.top + lane] = bad ? __builtin_nanf("") : list.i < 0 ? -__builtin_huge_valf() : scaled(list.v, s.m, it) - lnS;
     }
 }
 

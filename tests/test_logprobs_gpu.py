@@ -650,3 +650,16 @@ def test_derivatives_that_are_not_there_are_refused():
     with pytest.raises(ValueError, match="record"):
         make_fx(entropy)(x)
     assert torch.equal(entropy(x), policy.action_logprobs(x, a).entropy)
+
+
+@pytest.mark.parametrize("temperature", [4.0, 1e3, 1e6])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("v", [5, 512, 5000])
+def test_differences_beyond_float32_are_scaled_first(dtype, v, temperature):
+    """x - max may not fit where (x - max) / temperature does: lowest against largest values."""
+    x, a, allowed = make(6, v, dtype, v, k=3)
+    far = torch.finfo(dtype).max
+    x[:, 0], x[:, v - 1], x[:, 2] = far, -far, far * 0.75
+    a[:, 0], a[:, 1] = v - 1, 0
+    x[3] = -far
+    check(x, torch.ones_like(allowed), None, a, top=5, temperature=temperature, grads=False)
