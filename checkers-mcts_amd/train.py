@@ -242,7 +242,7 @@ def losses(net, x, pi, tv, autocast_dtype=None, with_penalty=True, entropy_weigh
     else:
         p, v = run(x.permute(0, 3, 1, 2))
     if entropy_weight:
-        z, p = p, F.softmax(p, dim=1)
+        z, p = p, F.softmax(p.float(), dim=1)
     p = p / p.sum(dim=1, keepdim=True)
     ce = -(pi * torch.log(p.clamp(1e-7, 1 - 1e-7))).sum(dim=1).mean()
     mse = F.mse_loss(v, tv)

@@ -663,3 +663,23 @@ def test_differences_beyond_float32_are_scaled_first(dtype, v, temperature):
     a[:, 0], a[:, 1] = v - 1, 0
     x[3] = -far
     check(x, torch.ones_like(allowed), None, a, top=5, temperature=temperature, grads=False)
+
+
+def test_losses_of_16_bit_logits_with_an_entropy_term():
+    """The softmax of the loss is float32 with the term as without it."""
+    from checkers_mcts_amd import train
+    from test_train_hip_gpu import make_batch
+    x, pi, tv = make_batch(64, 4)
+    z = (torch.randn((64, 512), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") * 3).bfloat16()
+
+    class Net:
+        policy_loss_weight = value_loss_weight = 1.0
+
+        def logits(self, x):
+            return z, tv * 0.5
+
+        def __call__(self, x):
+            return torch.softmax(z.float(), 1), tv * 0.5
+    without = train.losses(Net(), x, pi, tv, with_penalty=False)
+    with_term = train.losses(Net(), x, pi, tv, with_penalty=False, entropy_weight=0.25)
+    assert torch.equal(without[1], with_term[1]) and torch.equal(without[2], with_term[2])
