@@ -349,17 +349,18 @@ def train_nn(training_data, neural_network, **kwargs):
     # torch.optim.Adam (mixed-precision training, other network widths, and training sets smaller than one batch, which
     # the HIP step cannot fill)
     # (OPTIMIZER "adamw" / "adamw8" and ENTROPY_WEIGHT are the autograd path's: the HIP step has Keras' loss and Adam built in)
-    chosen = "TRAIN_BACKEND" in kwargs or optimizer != "adam" or entropy_weight != 0.0
+    chosen = optimizer != "adam" or entropy_weight != 0.0
     backend = kwargs.get("TRAIN_BACKEND", "hip" if (dev.type == "cuda" and amp == torch.float32 and net.num_kernels == 128
                                                      and BATCH_SIZE % 2 == 0 and not chosen) else "torch")
     if backend == "hip" and (optimizer != "adam" or entropy_weight):
         raise ValueError("TRAIN_BACKEND 'hip' has Adam and no entropy term: OPTIMIZER 'adamw' / 'adamw8' and ENTROPY_WEIGHT need 'torch'")
     if backend == "hip" and n_train < BATCH_SIZE:
         backend = "torch"               # fewer rows than one batch: every step would take the torch path and leave the HIP weights untouched
-    if backend == "torch" and not chosen and dev.type == "cuda":
+    if backend == "torch" and "TRAIN_BACKEND" not in kwargs and dev.type == "cuda":
         import warnings                 # never a silent change of backend (as for inference: pipeline.EvaluatorPlan)
         warnings.warn("train_nn: the optimisation step runs on PyTorch autograd / MIOpen, not on the hand-written kernels of ckr_train.hip "
-                      "(they take the 128-kernel network in float32, an even BATCH_SIZE and at least one full batch of rows); "
+                      "(they take the 128-kernel network in float32, an even BATCH_SIZE and at least one full batch of rows, with Keras' Adam "
+                      "and loss: no OPTIMIZER 'adamw' / 'adamw8', no ENTROPY_WEIGHT); "
                       "TRAIN_BACKEND='torch' selects this path explicitly", RuntimeWarning, stacklevel=2)
     hip = None
     if backend == "hip":

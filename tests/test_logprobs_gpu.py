@@ -683,3 +683,19 @@ def test_losses_of_16_bit_logits_with_an_entropy_term():
     without = train.losses(Net(), x, pi, tv, with_penalty=False)
     with_term = train.losses(Net(), x, pi, tv, with_penalty=False, entropy_weight=0.25)
     assert torch.equal(without[1], with_term[1]) and torch.equal(without[2], with_term[2])
+
+
+def test_leaving_the_hand_written_training_step_is_said(tmp_path, monkeypatch):
+    import warnings
+    from checkers_mcts_amd import train
+    from test_train_hip_gpu import make_batch
+    monkeypatch.chdir(tmp_path)
+    data = train.TrainingData(dense=make_batch(64, 6))
+    kw = dict(PATIENCE=5, MIN_DELTA=0, VAL_SPLIT=0.0, TRAINING_ITERATION=0, BATCH_SIZE=32, CLR_SS_COEFF=4, NN_BASE_LR=1e-4, NN_MAX_LR=1e-3, EPOCHS=1, NUM_KERNELS=128,
+              CONV_REG=1e-4, DENSE_REG=1e-4, POLICY_LOSS_WEIGHT=1.0, VALUE_LOSS_WEIGHT=1.0, SEED=1, MODEL_SUFFIX=".pt")
+    for more, said in ((dict(OPTIMIZER="adamw"), True), (dict(ENTROPY_WEIGHT=0.01), True), (dict(), False), (dict(OPTIMIZER="adamw8", TRAIN_BACKEND="torch"), False)):
+        with warnings.catch_warnings(record=True) as caught:
+            warnings.simplefilter("always")
+            train.train_nn(data, train.create_nn(**kw), **dict(kw, **more))
+        said_now = [str(w.message) for w in caught if issubclass(w.category, RuntimeWarning) and "hand-written" in str(w.message)]
+        assert bool(said_now) == said and all("OPTIMIZER" in m and "ENTROPY_WEIGHT" in m for m in said_now), (more, said_now)
