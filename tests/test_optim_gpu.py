@@ -891,3 +891,52 @@ def test_steps_of_16_bit_parameters_in_one_buffer_are_not_taken_for_changes(monk
     ps[2].grad = torch.zeros_like(ps[2])
     opt.step()
     assert followed == [[0, 1, 2]] and (ps[2].detach()[50:] > 4).all() and (ps[2].detach()[:50] < 1.01).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_training_step_of_both_operators(bits):
+    """Forward, loss, backward, clipping and step in one graph, replayed with new inputs between eager work of another optimiser: as eager steps."""
+    from checkers_mcts_amd import optim, policy
+    n, f, v = 64, 24, 512
+
+    def batch(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        x, move = torch.randn((n, f), generator=g, device="cuda"), torch.randint(0, v, (n,), generator=g, device="cuda")
+        legal = torch.rand((n, v), generator=g, device="cuda") < 0.05
+        legal[torch.arange(n, device="cuda"), move] = True
+        return x, move, legal
+
+    def build():
+        g = torch.Generator(device="cuda").manual_seed(0)
+        W = (torch.randn((v, f), generator=g, device="cuda") * 0.1).requires_grad_(True)
+        b = torch.zeros((v,), device="cuda").requires_grad_(True)
+        return (W, b), optim.AdamW([{"params": [W]}, {"params": [b], "weight_decay": 0.0}], lr=1e-2, state_bits=bits, max_norm=0.05, seed=2)
+
+    def train(params, opt, x, move, legal):
+        opt.zero_grad(set_to_none=False)
+        out = policy.action_logprobs(torch.addmm(params[1], x, params[0].t()), move, mask=legal, top=3)
+        loss = -out.logp.mean() - 0.01 * out.entropy.mean()
+        loss.backward()
+        opt.step()
+        return loss.detach(), out.top_action
+    mine, opt = build()
+    theirs, eager = build()
+    static = [t.clone() for t in batch(100)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        train(mine, opt, *static)
+    torch.cuda.current_stream().wait_stream(side)
+    train(theirs, eager, *batch(100))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = train(mine, opt, *static)
+    for rep in range(5):
+        for t, new in zip(static, batch(101 + rep)):
+            t.copy_(new)
+        graph.replay()
+        want = train(theirs, eager, *batch(101 + rep))                 # eager work between the replays
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(mine, theirs)) and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert torch.equal(opt.exp_avg_sq, eager.exp_avg_sq) and opt.steps.tolist() == eager.steps.tolist() == [rep + 2] * 2
