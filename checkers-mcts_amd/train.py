@@ -317,11 +317,12 @@ def train_nn(training_data, neural_network, **kwargs):
     lr_t = torch.tensor(float(clr.on_train_begin()), dtype=torch.float32, device=dev)
     # build-specific: OPTIMIZER "adam" (default, Keras' Adam) | "adamw" | "adamw8" (optim.AdamW, moments in 32 / 8 bits; WEIGHT_DECAY on the
     # kernels of conv / dense layers, clipping at MAX_GRAD_NORM), ENTROPY_WEIGHT (losses()), POLICY_METRICS (validation figures)
-    optimizer, entropy_weight = kwargs.get("OPTIMIZER", "adam"), float(kwargs.get("ENTROPY_WEIGHT", 0.0))
+    optimizer, entropy_weight = kwargs.get("OPTIMIZER", "adam"), float(kwargs.get("ENTROPY_WEIGHT") or 0.0)
     policy_metrics = bool(kwargs.get("POLICY_METRICS", False))
     if optimizer not in ("adam", "adamw", "adamw8"):
         raise ValueError("OPTIMIZER must be 'adam', 'adamw' or 'adamw8'")
-    if optimizer == "adam" and ("WEIGHT_DECAY" in kwargs or "MAX_GRAD_NORM" in kwargs):
+    weight_decay, max_norm = kwargs.get("WEIGHT_DECAY"), kwargs.get("MAX_GRAD_NORM")           # None: not given
+    if optimizer == "adam" and (weight_decay is not None or max_norm is not None):
         raise ValueError("WEIGHT_DECAY and MAX_GRAD_NORM belong to OPTIMIZER 'adamw' / 'adamw8'")
     if dev.type != "cuda" and (optimizer != "adam" or entropy_weight or policy_metrics):
         raise ValueError("OPTIMIZER 'adamw' / 'adamw8', ENTROPY_WEIGHT and POLICY_METRICS run on a GPU")
@@ -333,8 +334,8 @@ def train_nn(training_data, neural_network, **kwargs):
         kernels = [m.weight for m in net.modules() if isinstance(m, (torch.nn.Conv2d, torch.nn.Linear))]
         others = [p for p in net.parameters() if all(p is not k for k in kernels)]
         opt = AdamW([{"params": kernels}, {"params": others, "weight_decay": 0.0}], lr=lr_t, betas=(0.9, 0.999), eps=1e-7,
-                    weight_decay=float(kwargs.get("WEIGHT_DECAY", 0.01)), state_bits=8 if optimizer == "adamw8" else 32,
-                    max_norm=kwargs.get("MAX_GRAD_NORM"), seed=int(kwargs.get("SEED", 0)))
+                    weight_decay=0.01 if weight_decay is None else float(weight_decay), state_bits=8 if optimizer == "adamw8" else 32,
+                    max_norm=max_norm, seed=int(kwargs.get("SEED", 0)))
     # ModelCheckpoint's file, training_pipeline.py:139-141 (MODEL_SUFFIX '.pt': a torch state_dict instead of Keras HDF5)
     filepath = "data/model/Checkers_Model" + str(TRAINING_ITERATION + 1) + "_" + create_timestamp() + kwargs.get("MODEL_SUFFIX", ".h5")
     os.makedirs("data/model", exist_ok=True)

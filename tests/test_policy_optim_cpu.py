@@ -191,3 +191,14 @@ def test_saved_tensors_that_come_back_in_another_order_are_copied(lib, monkeypat
     addresses = {t.data_ptr() for t in keep}
     b = seen[-1]
     assert len(keep) == 4 and not addresses & {b.logits, b.actions, b.mask, b.stats} and (b.row_stride, b.mask_stride) == (7, 7)
+
+
+def test_train_nn_takes_none_for_what_is_not_given(tmp_path, monkeypatch):
+    from checkers_mcts_amd import train
+    monkeypatch.chdir(tmp_path)
+    data = [[torch.zeros(15, 8, 8).double().numpy(), torch.zeros(8, 8, 8).double().numpy() + 1 / 512, 0.0, 0.0]] * 4
+    kw = dict(PATIENCE=1, MIN_DELTA=0, VAL_SPLIT=0, TRAINING_ITERATION=0, BATCH_SIZE=2, CLR_SS_COEFF=4, NN_BASE_LR=1e-3, NN_MAX_LR=1e-2, EPOCHS=1, NUM_KERNELS=8,
+              CONV_REG=0.0, DENSE_REG=0.0, POLICY_LOSS_WEIGHT=1.0, VALUE_LOSS_WEIGHT=1.0, DEVICE="cpu", SEED=1, MODEL_SUFFIX=".pt",
+              OPTIMIZER="adam", MAX_GRAD_NORM=None, WEIGHT_DECAY=None, ENTROPY_WEIGHT=None)
+    history, _ = train.train_nn(data, train.create_nn(**kw), **kw)
+    assert len(history.history["loss"]) == 1
