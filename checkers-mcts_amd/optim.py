@@ -159,7 +159,7 @@ class AdamW:
         self._device_of, self._offset_of = [dev.index] * first, [where[id(p)] for p in self._every]
         # what the order of the states follows from: each group's parameters, their types and, where they are not row by row, how they lie
         self._arrangement = [[[str(p.dtype)] + ([] if p.is_contiguous() else [list(n) for n in _layout(p)]) for p in g["params"]] for g in groups]
-        self._guards = None                                            # of parameters and gradients that were found to be as above
+        self._guards, self._found = None, False                        # of parameters and gradients that were found to be as above
         self._adopt()
         self._streams = {torch.cuda.current_stream(dev).cuda_stream}
         torch.cuda.current_stream(dev).synchronize()                   # a step on any stream finds the states in place
@@ -210,7 +210,8 @@ class AdamW:
         try:
             if list(map(_STRIDE, gs)) == self._stride_of and list(map(_DTYPE, gs)) == self._type_of and list(map(_NBYTES, gs)) == self._nbytes_of \
                     and list(map(_DEVICE, gs)) == self._device_of and not any(map(_NEGATED, gs)):
-                self._guards = None if _make_guards is None else _make_guards(*ps, *gs)
+                self._guards = None if _make_guards is None or not self._found else _make_guards(*ps, *gs)      # (made in the second such step)
+                self._found = True
                 return array("Q", addresses), array("Q", map(_POINTER, gs)), keep
         except (TypeError, AttributeError, RuntimeError):              # None, or sparse
             pass

@@ -660,7 +660,9 @@ def test_a_parameter_seen_otherwise_beside_the_gradient_it_had_is_refused(native
     p = torch.arange(64.0, device="cuda").reshape(8, 8).requires_grad_(True)
     opt = optim.AdamW([p])
     p.grad = torch.arange(64.0, device="cuda").reshape(8, 8) - 30
-    opt.step()
+    for _ in range(3):
+        opt.step()
+    assert native == (opt._guards is not None) or optim._make_guards is None
     before = p.detach().clone()
     p.data = p.data.t()
     for again in (False, True):
@@ -669,10 +671,10 @@ def test_a_parameter_seen_otherwise_beside_the_gradient_it_had_is_refused(native
         assert p.grad.stride() == (8, 1) and p.stride() == (1, 8)
         with pytest.raises(ValueError):
             opt.step()
-        assert torch.equal(p.detach().t(), before) and int(opt.steps[0]) == 1
+        assert torch.equal(p.detach().t(), before) and int(opt.steps[0]) == 3
     p.data = p.data.t()                                               # as it was
     opt.step()
-    assert int(opt.steps[0]) == 2
+    assert int(opt.steps[0]) == 4
 
 
 @pytest.mark.parametrize("native", [True, False])
@@ -684,14 +686,15 @@ def test_a_parameter_of_another_type_at_the_same_address_is_refused(kept, native
     p = torch.ones(64, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
     opt = optim.AdamW([p])
     p.grad = torch.ones_like(p)
-    opt.step()
+    for _ in range(3):
+        opt.step()
     p.data = p.data.view(torch.float16)
     if not kept:
         p.grad = torch.ones(64, device="cuda", dtype=torch.float16)
     before = p.detach().clone()
     with pytest.raises(ValueError):
         opt.step()
-    assert torch.equal(p.detach(), before) and int(opt.steps[0]) == 1
+    assert torch.equal(p.detach(), before) and int(opt.steps[0]) == 3
 
 
 @pytest.mark.skipif(not hasattr(torch.Tensor, "grad_dtype"), reason="gradients have their parameters' type")
@@ -700,13 +703,14 @@ def test_a_gradient_of_another_type_is_refused():
     p = torch.ones(64, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
     opt = optim.AdamW([p])
     p.grad = torch.ones_like(p)
-    opt.step()
+    for _ in range(3):
+        opt.step()
     p.grad = None
     p.grad_dtype = torch.float16
     p.grad = torch.ones(64, device="cuda", dtype=torch.float16)
     with pytest.raises(ValueError):
         opt.step()
-    assert int(opt.steps[0]) == 1
+    assert int(opt.steps[0]) == 3
 
 
 @pytest.mark.parametrize("native", [True, False])
