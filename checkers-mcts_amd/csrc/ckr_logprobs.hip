@@ -9,9 +9,9 @@
 // An empty A: log p = -inf, H = 0, no alternatives, gradient 0.  NaN or +inf in A: NaN, and no alternatives.
 //
 // What bounds it: the bytes of the logits.  Forward, 4096 x 32768 bf16: 47 us = 5.7 TB/s (a large copy reaches 4.7-5.4), with 5 alternatives
-// 52 us; 8192 x 16384 float32: 94 us = 5.7 TB/s.  Gradient, 4096 x 32768 bf16: 96 us = 5.6 TB/s read and written.  A launch of few or
-// short rows is a chain of waits: one position (512) 5.4 us, 4096 positions 4.6 us, 8 us with 5 alternatives, one row of 131072 with 20
-// alternatives 9.5 + 5.5 us.  Six VALU operations an element, one of them the exponential: at 7.5 TB/s they would be the bound.
+// 52 us; 8192 x 16384 float32: 95 us = 5.6 TB/s.  Gradient, 4096 x 32768 bf16: 96 us = 5.6 TB/s read and written.  A launch of few or
+// short rows is a chain of waits: one position (512) with 8 alternatives 5.3 us, 4096 positions with 5 8.5 us, one row of 131072 with 20
+// alternatives 10.0 + 5.8 us.  Six VALU operations an element, one of them the exponential: at 7.5 TB/s they would be the bound.
 #include "ckr_host.h"
 #include "ckr_device.hip.h"
 #include <cmath>
@@ -425,8 +425,9 @@ __global__ __launch_bounds__(64) void k_logprobs_join(const Args A, int parts) {
 // ---- backward: a wavefront has BWD_PER_LANE elements a lane of one row ----------------------------------------------------------------
 constexpr int BWD_PER_LANE = 16, BWD_TILE = 64 * BWD_PER_LANE;
 // A gradient of this many bytes is stored past the caches (STREAMS), which keep no more than its end for whoever reads it.  Forward, backward and
-// a reduction of the gradient, bf16 rows of 32768, with the caches and past them: 128 MiB 129 and 152 us, 160 MiB 189 and 185 us, 206 MiB 247
-// and 237 us, 256 MiB 313 and 291 us.
+// a reduction of the gradient, bf16 rows of 32768, with the caches and past them: 128 MiB 148 and 167 us, 144 MiB 173 and 183 us, 160 MiB 206
+// and 198 us, 206 MiB 257 and 247 us, 256 MiB 320 and 303 us; with the product that a linear layer's gradient is in place of the reduction:
+// 160 MiB 175 and 166 us, 206 MiB 221 and 207 us, 256 MiB 260 and 243 us.
 constexpr long long STREAMED = 160ll << 20;
 
 template <typename T, int MASK, bool STREAMS>
@@ -489,11 +490,11 @@ __global__ __launch_bounds__(256) void k_logprobs_bwd(const Args A) {
 }
 
 // How a row is shared.  A row of one tile is a wavefront's.  A longer one is a workgroup's if its wavefronts get two tiles each: one of four
-// makes the row's list while other workgroups read (4096 x 32768 bf16: 47 us, with 5 alternatives 54 us, against 52 and 58 us of a wavefront per
-// row, lists by ranks; 8192 x 16384 float32: 93 and 102 us; but 16384 x 4096 bf16, half a tile each: 32 and 26 us), or if there are too few rows to
-// fill the card otherwise.  Rows fewer than about 1024 are cut into parts, which a second launch joins; where each has to make a list, a part
-// has a tile for each wavefront at least (one row of 131072 bf16 with 20 alternatives: 9.4 + 5.3 us for 16 parts, 8.6 + 7.2 us for 64; 517 rows of
-// 50001 fp16 under a mask with 10: 26.3 + 4.4 us at 1024 workgroups, 30.1 at 500, 27.7 + 5.4 us at 2560).
+// makes the row's list while other workgroups read (4096 x 32768 bf16: 47 us, with 5 alternatives 52 us, against 51 and 56 us of a wavefront per
+// row; 8192 x 16384 float32: 95 and 101 us against 101 and 106; but 16384 x 4096 bf16, half a tile each: 32 and 49 us against 25 and 36), or if
+// there are too few rows to fill the card otherwise.  Rows fewer than about 1024 are cut into parts, which a second launch joins; where each has
+// to make a list, a part has a tile for each wavefront at least (one row of 131072 bf16 with 20 alternatives: 9.8 + 5.8 us for 16 parts, 8.8 +
+// 7.7 us for 64; 517 rows of 50001 fp16 under a mask with 10: 26.3 + 4.3 us at 1024 workgroups, 30.2 at 500, 27.8 + 5.1 us at 2560).
 static bool split(const Args& A, int& parts, int& length) {
     constexpr long long GROUPS = 1024;
     const int span = 64 * (A.dtype == CKR_F32 ? Vec<float>::N : Vec<_Float16>::N);                // 64 vectors

@@ -87,6 +87,7 @@ class AdamW:
     max_norm      clip the gradients by their global norm (over all groups): g * min(1, max_norm / (norm + 1e-6)); the norm of the last
                   step is `grad_norm`, a float64 device scalar.
 
+    It is no torch.optim.Optimizer, which torch.optim.lr_scheduler asks for: a schedule sets param_groups[i]["lr"] or fills the device scalar.
     step() runs on the current stream and does not synchronise; it can be captured into a HIP graph (gradients then have to stay where
     they are: zero_grad(set_to_none=False)).  Steps of one optimiser must not run at the same time."""
 

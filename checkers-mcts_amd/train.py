@@ -316,7 +316,8 @@ def train_nn(training_data, neural_network, **kwargs):
     # the learning rate lives in a device tensor so that a captured step sees the cyclical schedule
     lr_t = torch.tensor(float(clr.on_train_begin()), dtype=torch.float32, device=dev)
     # build-specific: OPTIMIZER "adam" (default, Keras' Adam) | "adamw" | "adamw8" (optim.AdamW, moments in 32 / 8 bits; WEIGHT_DECAY on the
-    # kernels of conv / dense layers, clipping at MAX_GRAD_NORM), ENTROPY_WEIGHT (losses()), POLICY_METRICS (validation figures)
+    # kernels of conv / dense layers, beside the l2 penalty of CONV_REG / DENSE_REG, whose gradient goes through the moments and counts in the
+    # norm that MAX_GRAD_NORM clips), ENTROPY_WEIGHT (losses()), POLICY_METRICS (validation figures)
     optimizer, entropy_weight = kwargs.get("OPTIMIZER", "adam"), float(kwargs.get("ENTROPY_WEIGHT") or 0.0)
     policy_metrics = bool(kwargs.get("POLICY_METRICS", False))
     if optimizer not in ("adam", "adamw", "adamw8"):
