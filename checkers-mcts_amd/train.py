@@ -21,6 +21,7 @@ PATIENCE, MIN_DELTA); the best val_loss model is the one saved.
 import ctypes as C
 import os
 import pickle
+from contextlib import nullcontext
 from datetime import datetime
 
 import numpy as np
@@ -258,7 +259,7 @@ def policy_figures(net, x, pi, autocast_dtype=None):
     among the network's three best -- all over the legal moves -- and the rows that count.  A row without visits does not: a game that runs
     to its end leaves one, whose position has no legal move.  autocast_dtype: as in `losses`."""
     played, move = (pi > 0).any(dim=1), pi.argmax(dim=1)
-    with torch.autocast(device_type=x.device.type, dtype=autocast_dtype or torch.bfloat16, enabled=autocast_dtype not in (None, torch.float32)):
+    with torch.autocast(device_type=x.device.type, dtype=autocast_dtype) if autocast_dtype not in (None, torch.float32) else nullcontext():
         z = net.logits(x.permute(0, 3, 1, 2))[0]
     out = policy.action_logprobs(z, move, mask=policy.legal_from_features(x), top=3)
     hit = (out.top_action == move[:, None]).any(dim=1)

@@ -699,3 +699,21 @@ def test_leaving_the_hand_written_training_step_is_said(tmp_path, monkeypatch):
             train.train_nn(data, train.create_nn(**kw), **dict(kw, **more))
         said_now = [str(w.message) for w in caught if issubclass(w.category, RuntimeWarning) and "hand-written" in str(w.message)]
         assert bool(said_now) == said and all("OPTIMIZER" in m and "ENTROPY_WEIGHT" in m for m in said_now), (more, said_now)
+
+
+def test_policy_figures_take_the_precision_around_them():
+    from checkers_mcts_amd import train
+    from test_train_hip_gpu import make_batch
+    x, pi, _ = make_batch(8, 4)
+    seen = []
+
+    class Net:
+        def logits(self, x):
+            seen.append(torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else None)
+            return torch.zeros((8, 512), device="cuda"), None
+    train.policy_figures(Net(), x, pi)
+    train.policy_figures(Net(), x, pi, torch.float32)
+    train.policy_figures(Net(), x, pi, torch.bfloat16)
+    with torch.autocast("cuda", dtype=torch.float16):
+        train.policy_figures(Net(), x, pi)
+    assert seen == [None, None, torch.bfloat16, torch.float16]
